@@ -30,7 +30,10 @@ def build(verbose=False):
         sources=sources,
         build_directory=build_dir,
         extra_cflags=['-O3', '-std=c++17'],
-        extra_cuda_cflags=['-O3', '-std=c++17'],
+        # packed fp32 forms stay off: hipcc -O3 makes them out of scalar code
+        # and some of them have given wrong sums on this hardware
+        extra_cuda_cflags=['-O3', '-std=c++17', '-Xclang', '-target-feature',
+                           '-Xclang', '-packed-fp32-ops'],
         verbose=verbose,
         is_python_module=False,
         is_standalone=False,
