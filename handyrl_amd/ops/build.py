@@ -23,7 +23,8 @@ def build(verbose=False):
     # List sources explicitly: torch's hipify pass writes generated
     # `*_hip.hip` siblings next to the source, which a bare glob would pick
     # up on the next build (duplicate kernels / double op registration).
-    sources = [os.path.join(src_dir, 'ext.hip')]
+    sources = [os.path.join(src_dir, name)
+               for name in ('ext.hip', 'policy_loss.hip')]
 
     mod = cpp_extension.load(
         name='handyrl_amd_C',

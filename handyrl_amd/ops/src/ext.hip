@@ -1256,7 +1256,10 @@ static std::vector<torch::Tensor> masked_sample(
     return {action, prob};
 }
 
+void bind_policy_loss(pybind11::module& m);      // policy_loss.hip
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_policy_loss(m);
     m.def("target_scan", &target_scan,
           "fused TD/UPGO/V-Trace backward scan (targets, advantages)");
     m.def("masked_sample", &masked_sample,
