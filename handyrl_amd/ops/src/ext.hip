@@ -1257,9 +1257,11 @@ static std::vector<torch::Tensor> masked_sample(
 }
 
 void bind_policy_loss(pybind11::module& m);      // policy_loss.hip
+void bind_selective(pybind11::module& m);        // selective.hip
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     bind_policy_loss(m);
+    bind_selective(m);
     m.def("target_scan", &target_scan,
           "fused TD/UPGO/V-Trace backward scan (targets, advantages)");
     m.def("masked_sample", &masked_sample,

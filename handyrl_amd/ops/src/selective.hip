@@ -1,0 +1,1364 @@
+// Short causal convolution and selective state space scan over windows of
+// steps, and their single-step forms.
+//
+// Convolution over the OBSERVED steps (u: the carried inputs, then x):
+//   y_t = act(bias + sum_k w_k u_{t-K+1+k})
+// Scan, per channel c and state n, with d = softplus(dt + dt_bias):
+//   h_t = exp(d_t A) h_{t-1} + d_t B_t x_t,   y_t = (C_t . h_t + D x_t) silu(z_t)
+// Steps whose mask is 0 leave the carried state as it is and give y = 0;
+// nothing of what they hold is used.
+
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <hip/hip_runtime.h>
+
+namespace {
+
+using bf16 = __hip_bfloat16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_float<bf16>(float v) { return __float2bfloat16(v); }
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+template <typename T, int V>
+__device__ __forceinline__ void load_pack(const T* p, float* out) {
+    const Pack<T, V> raw = *(const Pack<T, V>*)p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = to_float(raw.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const float* in) {
+    Pack<T, V> raw;
+#pragma unroll
+    for (int i = 0; i < V; ++i) raw.v[i] = from_float<T>(in[i]);
+    *(Pack<T, V>*)p = raw;
+}
+
+// Four values of which the first `n` exist; the others read as 0.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int n, bool whole, float* out) {
+    if (whole && n >= 4) {
+        load_pack<T, 4>(p, out);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = i < n ? to_float(p[i]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int n, bool whole, const float* in) {
+    if (whole && n >= 4) {
+        store_pack<T, 4>(p, in);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = from_float<T>(in[i]);
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float sigmoid(float v) {
+    return __builtin_amdgcn_rcpf(1.f + exp2_fast(-kLog2e * v));
+}
+// max(v, 0) + log1p(e^-|v|); log1p(e) = 2 atanh(e / (2 + e)), whose series in
+// s = e / (2 + e) <= 1/3 ends below 2e-8 of the value after seven terms
+__device__ __forceinline__ float softplus(float v) {
+    const float e = exp2_fast(-kLog2e * fabsf(v));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float p = 1.f / 13.f;
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    return fmaxf(v, 0.f) + 2.f * s * p;
+}
+
+// ------------------------------------------------------------ convolution
+
+struct ConvArgs {
+    const void* x;              // (B, T, D), last axis dense
+    const float* w;             // (D, K)
+    const float* bias;          // (D) or null
+    const void* state;          // (B, K-1, D) dense, or null: zeros
+    const bool* mask;           // (B, T) or null
+    const void* dy;             // (B, T, D) dense
+    const void* dlast;          // (B, K-1, D) dense, or null
+    void* y;                    // (B, T, D); backward: dx
+    void* last;                 // (B, K-1, D); backward: dstate, or null
+    float* parts;               // backward: (nparts, K+1, D)
+    long batch, steps, xb, xt;
+    int width, tile, tiles, nparts, silu;
+};
+
+// The last K-1 observed inputs before t0, oldest first.
+template <typename T, int K, int V>
+__device__ __forceinline__ void conv_behind(const ConvArgs& p, long b, long t0, int c,
+                                            float (&win)[K - 1][V]) {
+    int need = K - 2;
+    const T* x = (const T*)p.x + b * p.xb + c;
+    for (long t = t0 - 1; t >= 0 && need >= 0; --t) {
+        if (p.mask && !p.mask[b * p.steps + t]) continue;
+        float v[V];
+        load_pack<T, V>(x + t * p.xt, v);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+            if (k == need)
+#pragma unroll
+                for (int i = 0; i < V; ++i) win[k][i] = v[i];
+        --need;
+    }
+    const int found = K - 2 - need;
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+        if (k > need) continue;
+        if (p.state) {
+            load_pack<T, V>((const T*)p.state + (b * (K - 1) + k + found) * p.width + c, win[k]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) win[k][i] = 0.f;
+        }
+    }
+}
+
+template <int K, int V>
+__device__ __forceinline__ void conv_weights(const ConvArgs& p, int c, float (&w)[K][V],
+                                             float (&bias)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][i] = p.w[(long)(c + i) * K + k];
+        bias[i] = p.bias ? p.bias[c + i] : 0.f;
+    }
+}
+
+// A lane walks V channels of one tile of steps with the window in registers.
+template <typename T, int K, int V>
+__global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
+{
+    const long lanes = p.width / V;
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    const int c = (int)(at % lanes) * V;
+    const long item = at / lanes;
+    const long b = item / p.tiles;
+    if (b >= p.batch) return;
+    const long t0 = (item % p.tiles) * p.tile;
+    const long t1 = t0 + p.tile < p.steps ? t0 + p.tile : p.steps;
+
+    float w[K][V], bias[V], win[K - 1][V];
+    conv_weights<K, V>(p, c, w, bias);
+    conv_behind<T, K, V>(p, b, t0, c, win);
+    const T* x = (const T*)p.x + b * p.xb + c;
+    T* y = (T*)p.y + b * p.steps * p.width + c;
+    for (long t = t0; t < t1; ++t) {
+        float out[V] = {};
+        if (!p.mask || p.mask[b * p.steps + t]) {
+            float v[V];
+            load_pack<T, V>(x + t * p.xt, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float s = bias[i];
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][i], win[k][i], s);
+                s = fmaf(w[K - 1][i], v[i], s);
+                out[i] = p.silu ? s * sigmoid(s) : s;
+#pragma unroll
+                for (int k = 0; k < K - 2; ++k) win[k][i] = win[k + 1][i];
+                win[K - 2][i] = v[i];
+            }
+        }
+        store_pack<T, V>(y + t * p.width, out);
+    }
+    if (t1 == p.steps) {
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+            store_pack<T, V>((T*)p.last + (b * (K - 1) + k) * p.width + c, win[k]);
+    }
+}
+
+// Backward: the lane walks its tile and K-1 observed steps behind it, so that
+// every input of the tile has met all steps that used it.  Each input of the
+// window has its gradient so far and its place: a step, -1 (another tile's),
+// or -2-j (the carried input j).
+template <typename T, int K, int V>
+__global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
+{
+    const long lanes = p.width / V;
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    const int c = (int)(at % lanes) * V;
+    const long part = at / lanes;
+    if (part >= p.nparts) return;
+
+    float w[K][V], bias[V], dw[K][V] = {}, db[V] = {};
+    conv_weights<K, V>(p, c, w, bias);
+    const long items = p.batch * p.tiles;
+    for (long item = part; item < items; item += p.nparts) {
+        const long b = item / p.tiles;
+        const long t0 = (item % p.tiles) * p.tile;
+        const long t1 = t0 + p.tile < p.steps ? t0 + p.tile : p.steps;
+        const T* x = (const T*)p.x + b * p.xb + c;
+        const T* dy = (const T*)p.dy + b * p.steps * p.width + c;
+        T* dx = (T*)p.y + b * p.steps * p.width + c;
+
+        float win[K - 1][V], acc[K - 1][V] = {};
+        long place[K - 1];
+        conv_behind<T, K, V>(p, b, t0, c, win);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) place[k] = t0 == 0 ? -2 - k : -1;
+
+        auto emit = [&](long to, const float (&g)[V]) {
+            if (to >= 0)
+                store_pack<T, V>(dx + to * p.width, g);
+            else if (to <= -2 && p.last)
+                store_pack<T, V>((T*)p.last + (b * (K - 1) - 2 - to) * p.width + c, g);
+        };
+        int ahead = 0;
+        for (long t = t0; t < p.steps && ahead < K - 1; ++t) {
+            const bool own = t < t1;
+            if (p.mask && !p.mask[b * p.steps + t]) {
+                const float zero[V] = {};
+                if (own) store_pack<T, V>(dx + t * p.width, zero);
+                continue;
+            }
+            if (!own) ++ahead;
+            float v[V], g[V], first[V];
+            load_pack<T, V>(x + t * p.xt, v);
+            load_pack<T, V>(dy + t * p.width, g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (p.silu) {
+                    float s = bias[i];
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][i], win[k][i], s);
+                    s = fmaf(w[K - 1][i], v[i], s);
+                    const float sg = sigmoid(s);
+                    g[i] *= sg * (1.f + s * (1.f - sg));
+                }
+                if (own) {
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) dw[k][i] = fmaf(g[i], win[k][i], dw[k][i]);
+                    dw[K - 1][i] = fmaf(g[i], v[i], dw[K - 1][i]);
+                    db[i] += g[i];
+                }
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) acc[k][i] = fmaf(w[k][i], g[i], acc[k][i]);
+                first[i] = acc[0][i];
+#pragma unroll
+                for (int k = 0; k < K - 2; ++k) {
+                    acc[k][i] = acc[k + 1][i];
+                    win[k][i] = win[k + 1][i];
+                }
+                acc[K - 2][i] = w[K - 1][i] * g[i];
+                win[K - 2][i] = v[i];
+            }
+            emit(place[0], first);
+#pragma unroll
+            for (int k = 0; k < K - 2; ++k) place[k] = place[k + 1];
+            place[K - 2] = own ? t : -1;
+        }
+        // what the window still holds of this tile ended in the carried inputs
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) {
+            if (place[k] == -1) continue;
+            if (p.dlast) {
+                float g[V];
+                load_pack<T, V>((const T*)p.dlast + (b * (K - 1) + k) * p.width + c, g);
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[k][i] += g[i];
+            }
+            emit(place[k], acc[k]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) p.parts[(part * (K + 1) + k) * p.width + c + i] = dw[k][i];
+        p.parts[(part * (K + 1) + K) * p.width + c + i] = db[i];
+    }
+}
+
+template <typename T, int K, int V>
+__global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs p)
+{
+    const long lanes = p.width / V;
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    const int c = (int)(at % lanes) * V;
+    const long b = at / lanes;
+    if (b >= p.batch) return;
+    float out[V] = {};
+    if (!p.mask || p.mask[b]) {
+        float w[K][V], bias[V], win[K - 1][V], v[V];
+        T* state = (T*)p.last + b * (K - 1) * p.width + c;
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) load_pack<T, V>(state + (long)k * p.width, win[k]);
+        load_pack<T, V>((const T*)p.x + b * p.xb + c, v);
+        conv_weights<K, V>(p, c, w, bias);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float s = bias[i];
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][i], win[k][i], s);
+            s = fmaf(w[K - 1][i], v[i], s);
+            out[i] = p.silu ? s * sigmoid(s) : s;
+        }
+#pragma unroll
+        for (int k = 0; k < K - 2; ++k) store_pack<T, V>(state + (long)k * p.width, win[k + 1]);
+        store_pack<T, V>(state + (long)(K - 2) * p.width, v);
+    }
+    store_pack<T, V>((T*)p.y + b * p.width + c, out);
+}
+
+// out[col] = sum over parts of parts[part][col], in a fixed order and 64 bits
+// (up to 1024 parts of either sign).  Columns are (k, d); out is (d, k) for
+// k < inner and goes to `rest` (d) for k == inner.
+__global__ __launch_bounds__(256) void column_sum_kernel(
+    const float* __restrict__ parts, long nparts, long width, int inner,
+    float* __restrict__ out, float* __restrict__ rest)
+{
+    const long cols = width * (inner + (rest ? 1 : 0));
+    const long col = (long)blockIdx.x * 16 + (threadIdx.x & 15);
+    const int slice = threadIdx.x >> 4;
+    double sum = 0;
+    if (col < cols)
+        for (long i = slice; i < nparts; i += 16) sum += parts[i * cols + col];
+    __shared__ double s[16][17];
+    s[slice][threadIdx.x & 15] = sum;
+    __syncthreads();
+    if (slice == 0 && col < cols) {
+        for (int i = 1; i < 16; ++i) sum += s[i][threadIdx.x & 15];
+        const long k = col / width, d = col % width;
+        if (k < inner) out[d * inner + k] = (float)sum;
+        else rest[d] = (float)sum;
+    }
+}
+
+// ------------------------------------------------------------------- scan
+
+struct ScanArgs {
+    const void *x, *dt, *z, *B, *C;     // z may be null
+    const float *A, *D, *bias;          // D, bias may be null
+    const float* state;                 // (B, D, N) or null: zeros
+    const bool* mask;                   // (B, T) or null
+    const void* dy;                     // (B, T, D) dense
+    const float* dlast;                 // (B, D, N) or null
+    void* y;                            // (B, T, D) dense
+    float* last;                        // (B, D, N)
+    float* ckpt;                        // (B, chunks, D, N) or null: h before each chunk
+    float *seg_h, *seg_d;               // (B, segs, D, N), (B, segs, D)
+    void *dx, *ddt, *dz;                // (B, T, D)
+    float *dBp, *dCp;                   // (tiles, B, T, G, N)
+    float *dAp, *dDp;                   // (B segs, D, N), (B segs, 2, D): dD, dbias
+    float* dstate;                      // (B, D, N) or null
+    long batch, steps, chunks;
+    long xb, xt, db, dt_, zb, zt, Bb, Bt, Bg, Cb, Ct, Cg;
+    int width, states, groups, per, tiles, segs, seg_chunks;
+    int softplus, vec_d, vec_n, vec_b;
+};
+
+constexpr int TC = 16;          // steps of a chunk
+
+// Sum over the L lanes of a channel; every lane gets it.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+        0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int L> __device__ __forceinline__ float channel_sum(float v) {
+    if (L > 1) v += dpp<0xB1>(v);       // quad lanes 1 0 3 2
+    if (L > 2) v += dpp<0x4E>(v);       // quad lanes 2 3 0 1
+    if (L > 4) v += dpp<0x141>(v);      // the half row backwards
+    if (L > 8) v += dpp<0x140>(v);      // the row backwards
+    return v;
+}
+
+// Which rows, channels and steps a block has: 256 threads take 256/L channels
+// of one group, L lanes a channel and four states a lane.
+template <int L> struct Place {
+    static constexpr int CB = 256 / L, NP = 4 * L;
+    long b;
+    int g, seg, tile, c0, nc;           // first channel, how many
+    int c, n0, nn;                      // this lane's channel in the block, its states
+    bool live;
+    __device__ __forceinline__ Place(const ScanArgs& p) {
+        long at = blockIdx.x;
+        tile = (int)(at % p.tiles); at /= p.tiles;
+        g = (int)(at % p.groups); at /= p.groups;
+        seg = (int)(at % p.segs);
+        b = at / p.segs;
+        c0 = g * p.per + tile * CB;
+        nc = min(CB, p.per - tile * CB);
+        c = threadIdx.x / L;
+        n0 = 4 * (threadIdx.x % L);
+        live = c < nc;
+        nn = live ? min(4, max(0, p.states - n0)) : 0;
+    }
+    __device__ __forceinline__ long state_at(const ScanArgs& p, long row) const {
+        return (row * p.width + c0 + c) * p.states + n0;
+    }
+};
+
+// One thread's part of the values of a chunk: four channels of a step at a time.
+template <int L> struct Part {
+    static constexpr int groups = TC * (256 / L) / 4;
+    static constexpr int count = (groups + 255) / 256;
+    int t, c;
+    bool in;                            // the part exists
+    __device__ __forceinline__ Part(int k) {
+        const int at = threadIdx.x + 256 * k;
+        in = at < groups;
+        t = at / (256 / L / 4);
+        c = 4 * (at % (256 / L / 4));
+    }
+};
+
+template <typename T, int L>
+__device__ __forceinline__ void stage_bc(const ScanArgs& p, const Place<L>& at, long t0,
+                                         float (*sB)[4 * L], float (*sC)[4 * L]) {
+    const int tid = threadIdx.x;
+    if (tid < TC * L) {
+        const int t = tid / L, n = 4 * (tid % L);
+        float vb[4] = {}, vc[4] = {};
+        const long s = t0 + t;
+        if (s < p.steps && (!p.mask || p.mask[at.b * p.steps + s])) {
+            load4((const T*)p.B + at.b * p.Bb + s * p.Bt + at.g * p.Bg + n, p.states - n, p.vec_b, vb);
+            load4((const T*)p.C + at.b * p.Cb + s * p.Ct + at.g * p.Cg + n, p.states - n, p.vec_b, vc);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sB[t][n + i] = vb[i];
+            sC[t][n + i] = vc[i];
+        }
+    }
+}
+
+// x and d = softplus(dt + bias) of a thread's part; zeros where nothing is.
+template <typename T, int L>
+__device__ __forceinline__ bool load_xd(const ScanArgs& p, const Place<L>& at, const Part<L>& q,
+                                        long t0, float* x, float* d, float* raw) {
+    const long s = t0 + q.t;
+    const int n = at.nc - q.c;
+    const bool on = q.in && n > 0 && s < p.steps && (!p.mask || p.mask[at.b * p.steps + s]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = d[i] = raw[i] = 0.f;
+    if (on) {
+        const int c = at.c0 + q.c;
+        load4((const T*)p.x + at.b * p.xb + s * p.xt + c, n, p.vec_d, x);
+        load4((const T*)p.dt + at.b * p.db + s * p.dt_ + c, n, p.vec_d, raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >= n) continue;
+            if (p.bias) raw[i] += p.bias[c + i];
+            d[i] = p.softplus ? softplus(raw[i]) : raw[i];
+        }
+    }
+    return on;
+}
+
+template <int L>
+__device__ __forceinline__ void load_rates(const ScanArgs& p, const Place<L>& at, float* A2) {
+    load4(p.A + (long)(at.c0 + at.c) * p.states + at.n0, at.nn, p.vec_n, A2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A2[i] *= kLog2e;
+}
+
+// LOCAL: the segment's own end from a zero start, and its sum of d, for the
+// segments behind it.  Otherwise the outputs, from the state before the
+// segment: the carried one moved through the segments before.
+template <typename T, int L, bool LOCAL>
+__global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
+{
+    const Place<L> at(p);
+    __shared__ float2 sdu[TC][256 / L];
+    __shared__ float sB[TC][4 * L], sC[TC][4 * L], sy[TC][256 / L];
+
+    float A2[4], h[4] = {}, total = 0.f;
+    load_rates<L>(p, at, A2);
+    if (!LOCAL) {
+        if (p.state && at.nn > 0) load4(p.state + at.state_at(p, at.b), at.nn, p.vec_n, h);
+        for (int s = 0; s < at.seg && at.nn > 0; ++s) {
+            const long row = at.b * p.segs + s;
+            float e[4];
+            load4(p.seg_h + at.state_at(p, row), at.nn, p.vec_n, e);
+            const float d = p.seg_d[row * p.width + at.c0 + at.c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_fast(A2[i] * d), h[i], e[i]);
+        }
+    }
+    const long k0 = (long)at.seg * p.seg_chunks;
+    const long k1 = min(k0 + p.seg_chunks, p.chunks);
+    for (long k = k0; k < k1; ++k) {
+        const long t0 = k * TC;
+        float x[Part<L>::count][4];
+        bool on[Part<L>::count];
+#pragma unroll
+        for (int j = 0; j < Part<L>::count; ++j) {
+            const Part<L> q(j);
+            float d[4], raw[4];
+            on[j] = load_xd<T, L>(p, at, q, t0, x[j], d, raw);
+            if (q.in)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sdu[q.t][q.c + i] = make_float2(d[i], d[i] * x[j][i]);
+        }
+        stage_bc<T, L>(p, at, t0, sB, sC);
+        __syncthreads();
+        if (!LOCAL && p.ckpt && at.nn > 0)
+            store4(p.ckpt + at.state_at(p, at.b * p.chunks + k), at.nn, p.vec_n, h);
+        const int n = (int)min((long)TC, p.steps - t0);
+#pragma unroll 4
+        for (int t = 0; t < n; ++t) {
+            const float2 v = sdu[t][at.c];
+            float y = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = fmaf(exp2_fast(A2[i] * v.x), h[i], v.y * sB[t][at.n0 + i]);
+                if (!LOCAL) y = fmaf(sC[t][at.n0 + i], h[i], y);
+            }
+            if (LOCAL) {
+                total += v.x;
+            } else {
+                y = channel_sum<L>(y);
+                if (at.n0 == 0) sy[t][at.c] = y;
+            }
+        }
+        __syncthreads();
+        if (LOCAL) continue;
+#pragma unroll
+        for (int j = 0; j < Part<L>::count; ++j) {
+            const Part<L> q(j);
+            const long s = t0 + q.t;
+            if (!q.in || q.c >= at.nc || s >= p.steps) continue;
+            const int n = at.nc - q.c, c = at.c0 + q.c;
+            float y[4] = {};
+            if (on[j]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = sy[q.t][q.c + i];
+                    if (p.D && i < n) y[i] = fmaf(p.D[c + i], x[j][i], y[i]);
+                }
+                if (p.z) {
+                    float z[4];
+                    load4((const T*)p.z + at.b * p.zb + s * p.zt + c, n, p.vec_d, z);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] *= z[i] * sigmoid(z[i]);
+                }
+            }
+            store4((T*)p.y + (at.b * p.steps + s) * p.width + c, n, p.vec_d, y);
+        }
+    }
+    if (LOCAL) {
+        const long row = at.b * p.segs + at.seg;
+        if (at.nn > 0) store4(p.seg_h + at.state_at(p, row), at.nn, p.vec_n, h);
+        if (at.live && at.n0 == 0) p.seg_d[row * p.width + at.c0 + at.c] = total;
+    } else if (at.seg == p.segs - 1 && at.nn > 0) {
+        store4(p.last + at.state_at(p, at.b), at.nn, p.vec_n, h);
+    }
+}
+
+// Backward.  With g_t the gradient of C.h + D x and lam_t that of h_t:
+//   lam_t = C_t g_t + carry,  carry <- exp(d_t A) lam_t
+// LOCAL: a segment's carry from a zero one behind it.  Otherwise the
+// gradients: h is walked again from the chunk's checkpoint and kept in
+// registers with exp(d A), then the chunk is walked backwards.
+template <typename T, int L, bool LOCAL>
+__global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs p)
+{
+    constexpr int CB = 256 / L, NP = 4 * L;
+    const Place<L> at(p);
+    __shared__ float2 sdx[TC][CB];                      // d, x
+    __shared__ float sg[TC][CB], sB[TC][NP], sC[TC][NP];
+    __shared__ float2 ss[LOCAL ? 1 : TC][CB];           // sum lam B, sum A2 a h lam
+    __shared__ float sy[LOCAL ? 1 : TC][CB];
+    __shared__ float2 sbc[LOCAL ? 1 : 4][TC][NP];       // each wave's dB, dC
+
+    float A2[4], lam[4] = {}, dA[4] = {}, total = 0.f;
+    float dD[4] = {}, dbias[4] = {};
+    load_rates<L>(p, at, A2);
+    if (!LOCAL) {
+        if (p.dlast && at.nn > 0) load4(p.dlast + at.state_at(p, at.b), at.nn, p.vec_n, lam);
+        for (int s = p.segs - 1; s > at.seg && at.nn > 0; --s) {
+            const long row = at.b * p.segs + s;
+            float e[4];
+            load4(p.seg_h + at.state_at(p, row), at.nn, p.vec_n, e);
+            const float d = p.seg_d[row * p.width + at.c0 + at.c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lam[i] = fmaf(exp2_fast(A2[i] * d), lam[i], e[i]);
+        }
+    }
+    const long k0 = (long)at.seg * p.seg_chunks;
+    const long k1 = min(k0 + p.seg_chunks, p.chunks);
+    for (long k = k1 - 1; k >= k0; --k) {
+        const long t0 = k * TC;
+        constexpr int NQ = Part<L>::count;
+        float x[NQ][4], raw[NQ][4], z[NQ][4], dy[NQ][4];
+        bool on[NQ];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            const Part<L> q(j);
+            float d[4];
+            on[j] = load_xd<T, L>(p, at, q, t0, x[j], d, raw[j]);
+            const int c = at.c0 + q.c, n = at.nc - q.c;
+            const long s = t0 + q.t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dy[j][i] = z[j][i] = 0.f;
+            if (on[j]) {
+                load4((const T*)p.dy + (at.b * p.steps + s) * p.width + c, n, p.vec_d, dy[j]);
+                if (p.z) load4((const T*)p.z + at.b * p.zb + s * p.zt + c, n, p.vec_d, z[j]);
+            }
+            if (q.in)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sdx[q.t][q.c + i] = make_float2(d[i], x[j][i]);
+                    sg[q.t][q.c + i] = p.z ? dy[j][i] * z[j][i] * sigmoid(z[j][i]) : dy[j][i];
+                }
+        }
+        stage_bc<T, L>(p, at, t0, sB, sC);
+        __syncthreads();
+
+        if (LOCAL) {
+#pragma unroll 4
+            for (int t = TC - 1; t >= 0; --t) {
+                const float d = sdx[t][at.c].x, g = sg[t][at.c];
+                total += d;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    lam[i] = exp2_fast(A2[i] * d) * fmaf(sC[t][at.n0 + i], g, lam[i]);
+            }
+            __syncthreads();
+            continue;
+        } else {
+            float hs[TC + 1][4], a[TC][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) hs[0][i] = 0.f;
+            if (at.nn > 0)
+                load4(p.ckpt + at.state_at(p, at.b * p.chunks + k), at.nn, p.vec_n, hs[0]);
+#pragma unroll
+            for (int t = 0; t < TC; ++t) {
+                const float2 v = sdx[t][at.c];
+                const float du = v.x * v.y;
+                float y = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a[t][i] = exp2_fast(A2[i] * v.x);
+                    hs[t + 1][i] = fmaf(a[t][i], hs[t][i], du * sB[t][at.n0 + i]);
+                    y = fmaf(sC[t][at.n0 + i], hs[t + 1][i], y);
+                }
+                if (p.z) {
+                    y = channel_sum<L>(y);
+                    if (at.n0 == 0) sy[t][at.c] = y;
+                }
+            }
+#pragma unroll
+            for (int t = TC - 1; t >= 0; --t) {
+                const float2 v = sdx[t][at.c];
+                const float du = v.x * v.y, g = sg[t][at.c];
+                float s1 = 0.f, s2 = 0.f, vb[4], vc[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float l = fmaf(sC[t][at.n0 + i], g, lam[i]);
+                    vc[i] = g * hs[t + 1][i];
+                    vb[i] = l * du;
+                    s1 = fmaf(l, sB[t][at.n0 + i], s1);
+                    lam[i] = a[t][i] * l;
+                    const float ah = lam[i] * hs[t][i];
+                    s2 = fmaf(A2[i], ah, s2);
+                    dA[i] = fmaf(v.x, ah, dA[i]);
+                }
+                s1 = channel_sum<L>(s1);
+                s2 = channel_sum<L>(s2);
+                if (at.n0 == 0) ss[t][at.c] = make_float2(s1, s2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int o = L; o < 64; o <<= 1) {
+                        vb[i] += __shfl_xor(vb[i], o);
+                        vc[i] += __shfl_xor(vc[i], o);
+                    }
+                }
+                if ((threadIdx.x & 63) < L)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sbc[threadIdx.x >> 6][t][at.n0 + i] = make_float2(vb[i], vc[i]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                const Part<L> q(j);
+                const long s = t0 + q.t;
+                if (!q.in || q.c >= at.nc || s >= p.steps) continue;
+                const int n = at.nc - q.c, c = at.c0 + q.c;
+                float dx[4] = {}, dd[4] = {}, dz[4] = {};
+                if (on[j]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 v = ss[q.t][q.c + i];
+                        const float g = sg[q.t][q.c + i], Dc = p.D && i < n ? p.D[c + i] : 0.f;
+                        dx[i] = fmaf(sdx[q.t][q.c + i].x, v.x, Dc * g);
+                        dd[i] = fmaf(x[j][i], v.x, kLn2 * v.y);
+                        if (p.softplus) dd[i] *= sigmoid(raw[j][i]);
+                        dD[i] = fmaf(g, x[j][i], dD[i]);
+                        dbias[i] += dd[i];
+                        if (p.z) {
+                            const float sg_ = sigmoid(z[j][i]);
+                            dz[i] = dy[j][i] * fmaf(Dc, x[j][i], sy[q.t][q.c + i]) *
+                                    sg_ * (1.f + z[j][i] * (1.f - sg_));
+                        }
+                    }
+                }
+                const long to = (at.b * p.steps + s) * p.width + c;
+                store4((T*)p.dx + to, n, p.vec_d, dx);
+                store4((T*)p.ddt + to, n, p.vec_d, dd);
+                if (p.z) store4((T*)p.dz + to, n, p.vec_d, dz);
+            }
+            for (int e = threadIdx.x; e < TC * NP; e += 256) {
+                const int t = e / NP, n = e % NP;
+                const long s = t0 + t;
+                if (n >= p.states || s >= p.steps) continue;
+                const long to = (((at.tile * p.batch + at.b) * p.steps + s) * p.groups + at.g) *
+                                p.states + n;
+                float vb = 0.f, vc = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    vb += sbc[w][t][n].x;
+                    vc += sbc[w][t][n].y;
+                }
+                p.dBp[to] = vb;
+                p.dCp[to] = vc;
+            }
+            __syncthreads();
+        }
+    }
+    const long row = at.b * p.segs + at.seg;
+    if (LOCAL) {
+        if (at.nn > 0) store4(p.seg_h + at.state_at(p, row), at.nn, p.vec_n, lam);
+        if (at.live && at.n0 == 0) p.seg_d[row * p.width + at.c0 + at.c] = total;
+    } else {
+        if (at.seg == 0 && p.dstate && at.nn > 0)
+            store4(p.dstate + at.state_at(p, at.b), at.nn, p.vec_n, lam);
+        if (at.nn > 0) store4(p.dAp + at.state_at(p, row), at.nn, p.vec_n, dA);
+        // dD and dbias: a thread has its four channels over its steps of each chunk
+        float* fold = (float*)sdx;
+        constexpr int rows = 256 / (CB / 4);
+        const int c4 = 4 * (threadIdx.x % (CB / 4)), r = threadIdx.x / (CB / 4);
+        for (int which = 0; which < 2; ++which) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r < TC) fold[r * CB + c4 + i] = which ? dbias[i] : dD[i];
+            __syncthreads();
+            for (int c = threadIdx.x; c < at.nc; c += 256) {
+                float s = 0.f;
+                for (int i = 0; i < (rows < TC ? rows : TC); ++i) s += fold[i * CB + c];
+                p.dDp[(row * 2 + which) * p.width + at.c0 + c] = s;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Sums dB and dC over the channel tiles and rounds them once.
+template <typename T>
+__global__ __launch_bounds__(256) void tile_sum_kernel(
+    const float* __restrict__ parts, int tiles, long n, T* __restrict__ out)
+{
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.f;
+    for (int k = 0; k < tiles; ++k) s += parts[k * n + i];
+    out[i] = from_float<T>(s);
+}
+
+struct StepArgs {
+    const void *x, *dt, *z, *B, *C;
+    const float *A, *D, *bias;
+    const bool* mask;
+    float* state;
+    void* y;
+    long batch, xb, db, zb, Bb, Bg, Cb, Cg;
+    int width, states, groups, per, softplus, vec_n, vec_b;
+};
+
+// One step: four states a lane, L lanes a channel, the state in place.
+template <typename T, int L>
+__global__ __launch_bounds__(256) void scan_step_kernel(StepArgs p)
+{
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    const int n0 = 4 * (int)(at % L);
+    const long row = at / L;                            // (b, channel)
+    const long b = row / p.width;
+    const int c = (int)(row % p.width), g = c / p.per;
+    const bool in = b < p.batch, on = in && (!p.mask || p.mask[b]);
+    const int nn = on ? min(4, max(0, p.states - n0)) : 0;
+    float y = 0.f, x = 0.f;
+    if (on) {
+        float raw = to_float(((const T*)p.dt)[b * p.db + c]);
+        x = to_float(((const T*)p.x)[b * p.xb + c]);
+        if (p.bias) raw += p.bias[c];
+        const float d = p.softplus ? softplus(raw) : raw, du = d * x;
+        if (nn > 0) {
+            float h[4], A[4], vb[4], vc[4];
+            load4(p.state + row * p.states + n0, nn, p.vec_n, h);
+            load4(p.A + (long)c * p.states + n0, nn, p.vec_n, A);
+            load4((const T*)p.B + b * p.Bb + g * p.Bg + n0, nn, p.vec_b, vb);
+            load4((const T*)p.C + b * p.Cb + g * p.Cg + n0, nn, p.vec_b, vc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = fmaf(exp2_fast(A[i] * kLog2e * d), h[i], du * vb[i]);
+                y = fmaf(vc[i], h[i], y);
+            }
+            store4(p.state + row * p.states + n0, nn, p.vec_n, h);
+        }
+    }
+    y = channel_sum<L>(y);
+    if (in && n0 == 0) {
+        if (on) {
+            if (p.D) y = fmaf(p.D[c], x, y);
+            if (p.z) {
+                const float z = to_float(((const T*)p.z)[b * p.zb + c]);
+                y *= z * sigmoid(z);
+            }
+        }
+        ((T*)p.y)[row] = from_float<T>(on ? y : 0.f);
+    }
+}
+
+// ------------------------------------------------------------------- host
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+// The kernels read the last axis dense; anything else is laid out anew.
+Tensor dense_last(const Tensor& t) {
+    return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+bool aligned(const Tensor& t, int v) {
+    if ((uintptr_t)t.data_ptr() % (v * t.element_size())) return false;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) % v) return false;
+    return true;
+}
+
+void check_like(const char* op, const char* name, const Tensor& t, const Tensor& x,
+                torch::ScalarType type, at::IntArrayRef shape)
+{
+    TORCH_CHECK_VALUE(t.device() == x.device(), op, ": ", name, " is on ", t.device(),
+                      ", x on ", x.device());
+    TORCH_CHECK_VALUE(t.scalar_type() == type, op, ": ", name, " must be ", type, ", got ",
+                      t.scalar_type());
+    TORCH_CHECK_VALUE(t.sizes() == shape, op, ": ", name, " must have shape ", shape, ", got ",
+                      t.sizes());
+}
+
+void check_x(const char* op, const Tensor& x, int64_t dim)
+{
+    TORCH_CHECK_VALUE(x.is_cuda(), op, ": x must be on the GPU");
+    TORCH_CHECK_VALUE(x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16,
+                      op, ": x must be float32 or bfloat16, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() == dim && x.size(-1) >= 1, op, ": x must be ",
+                      dim == 3 ? "(batch, steps, channels)" : "(batch, channels)", ", got ",
+                      x.sizes());
+    TORCH_CHECK_VALUE(x.size(-1) < (1L << 24), op, ": too many channels");
+}
+
+// (B, T), or (B, T, 1), of truth values or numbers: 0 is unobserved.
+Tensor as_mask(const char* op, const OptTensor& mask, const Tensor& x)
+{
+    if (!mask) return Tensor();
+    auto want = x.sizes().slice(0, x.dim() - 1);
+    auto m = *mask;
+    if (m.dim() == x.dim() && m.size(-1) == 1) m = m.squeeze(-1);
+    TORCH_CHECK_VALUE(m.device() == x.device(), op, ": mask is on ", m.device(), ", x on ",
+                      x.device());
+    TORCH_CHECK_VALUE(m.sizes() == want, op, ": mask must have shape ", want, ", got ",
+                      mask->sizes());
+    return (m.scalar_type() == torch::kBool ? m : m.ne(0)).contiguous();
+}
+
+int64_t blocks_for(int64_t threads, const char* op)
+{
+    const int64_t n = (threads + 255) / 256;
+    TORCH_CHECK_VALUE(n < (1LL << 31), op, ": too large for one launch");
+    return n;
+}
+
+template <typename F> void by_type(const Tensor& x, F f)
+{
+    if (x.scalar_type() == torch::kBFloat16) f(bf16());
+    else f(float());
+}
+template <int N> struct Const { static constexpr int value = N; };
+
+// A step changes the state behind torch's back: tell autograd's version check.
+void moved_on(const Tensor& state) {
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
+
+// ---- convolution
+
+template <typename F> void by_taps(int64_t taps, F f)
+{
+    if (taps == 2) f(Const<2>());
+    else if (taps == 3) f(Const<3>());
+    else f(Const<4>());
+}
+
+template <typename F> void by_conv(const Tensor& x, int64_t taps, bool wide, F f)
+{
+    by_type(x, [&](auto t) {
+        using T = decltype(t);
+        by_taps(taps, [&](auto k) {
+            if (wide) f(t, k, Const<16 / sizeof(T)>());
+            else f(t, k, Const<1>());
+        });
+    });
+}
+
+const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const float* fptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+const bool* mptr(const Tensor& t) { return t.defined() ? t.data_ptr<bool>() : nullptr; }
+
+ConvArgs conv_args(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& state,
+                   const Tensor& mask, bool silu)
+{
+    ConvArgs p{};
+    p.x = ptr(x); p.w = fptr(w); p.bias = fptr(bias); p.state = ptr(state); p.mask = mptr(mask);
+    p.batch = x.size(0); p.steps = x.dim() == 3 ? x.size(1) : 1;
+    p.xb = x.stride(0); p.xt = x.dim() == 3 ? x.stride(1) : 0;
+    p.width = (int)x.size(-1); p.silu = silu;
+    return p;
+}
+
+// Whether all of them can be read 16 bytes at a time.
+bool conv_wide(const Tensor& x, std::initializer_list<Tensor> others)
+{
+    const int v = 16 / x.element_size();
+    bool ok = x.size(-1) % v == 0 && aligned(x, v);
+    for (auto& t : others) ok = ok && (!t.defined() || aligned(t, v));
+    return ok;
+}
+
+std::vector<Tensor> conv_forward(const Tensor& x, const Tensor& w, const Tensor& bias,
+                                 const Tensor& state, const Tensor& mask, bool silu)
+{
+    const c10::DeviceGuard guard(x.device());
+    auto stream = at::cuda::getCurrentCUDAStream();
+    const int64_t taps = w.size(1);
+    auto y = torch::empty(x.sizes(), x.options());
+    auto last = torch::empty({x.size(0), taps - 1, x.size(2)}, x.options());
+    ConvArgs p = conv_args(x, w, bias, state, mask, silu);
+    if (p.batch == 0 || p.steps == 0) {
+        if (state.defined()) last.copy_(state); else last.zero_();
+        return {y, last};
+    }
+    p.y = y.data_ptr(); p.last = last.data_ptr();
+    p.tile = 16;
+    p.tiles = (int)((p.steps + p.tile - 1) / p.tile);
+    by_conv(x, taps, conv_wide(x, {state}), [&](auto t, auto k, auto v) {
+        const int64_t n = blocks_for(p.batch * p.tiles * (p.width / v.value), "causal_conv");
+        hipLaunchKernelGGL((conv_fwd_kernel<decltype(t), decltype(k)::value, decltype(v)::value>),
+                           dim3(n), dim3(256), 0, stream, p);
+    });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    return {y, last};
+}
+
+class CausalConv : public torch::autograd::Function<CausalConv> {
+public:
+    static torch::autograd::variable_list forward(
+        torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w,
+        const OptTensor& bias_in, const OptTensor& state_in, const OptTensor& mask_in, bool silu)
+    {
+        const auto bias = bias_in.value_or(Tensor()), state = state_in.value_or(Tensor()),
+                   mask = mask_in.value_or(Tensor());
+        ctx->save_for_backward({x, w, bias, state, mask});
+        ctx->saved_data["silu"] = silu;
+        return conv_forward(x, w, bias, state, mask, silu);
+    }
+
+    static torch::autograd::variable_list backward(
+        torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        TORCH_CHECK(!at::GradMode::is_enabled(),
+                    "causal_conv: its gradients are not differentiable again");
+        auto saved = ctx->get_saved_variables();
+        const auto &x = saved[0], &w = saved[1], &bias = saved[2], &state = saved[3];
+        const c10::DeviceGuard guard(x.device());
+        auto stream = at::cuda::getCurrentCUDAStream();
+        const int64_t taps = w.size(1);
+        auto dy = grads[0].defined() ? grads[0].contiguous()
+                                     : torch::zeros(x.sizes(), x.options());
+        auto dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        auto dx = torch::empty(x.sizes(), x.options());
+        auto dw = torch::empty(w.sizes(), w.options());
+        auto db = bias.defined() ? torch::empty({x.size(2)}, w.options()) : Tensor();
+        auto dstate = state.defined() ? torch::empty(state.sizes(), x.options()) : Tensor();
+        ConvArgs p = conv_args(x, w, bias, state, saved[4], ctx->saved_data["silu"].toBool());
+        p.dy = ptr(dy); p.dlast = ptr(dlast); p.y = dx.data_ptr();
+        p.last = dstate.defined() ? dstate.data_ptr() : nullptr;
+        if (p.batch == 0 || p.steps == 0) {
+            dw.zero_();
+            if (db.defined()) db.zero_();
+            if (dstate.defined()) {
+                if (dlast.defined()) dstate.copy_(dlast); else dstate.zero_();
+            }
+            return {dx, dw, db, dstate, Tensor(), Tensor()};
+        }
+        p.tile = 16;
+        p.tiles = (int)((p.steps + p.tile - 1) / p.tile);
+        p.nparts = (int)std::min<int64_t>(p.batch * p.tiles, 256);
+        auto parts = torch::empty({p.nparts, taps + 1, x.size(2)}, w.options());
+        p.parts = parts.data_ptr<float>();
+        by_conv(x, taps, conv_wide(x, {state, dy, dlast}), [&](auto t, auto k, auto v) {
+            const int64_t n = blocks_for((int64_t)p.nparts * (p.width / v.value), "causal_conv");
+            hipLaunchKernelGGL((conv_bwd_kernel<decltype(t), decltype(k)::value,
+                                decltype(v)::value>), dim3(n), dim3(256), 0, stream, p);
+        });
+        auto rest = db.defined() ? db : torch::empty({x.size(2)}, w.options());
+        const int64_t cols = (taps + 1) * x.size(2);
+        hipLaunchKernelGGL(column_sum_kernel, dim3((cols + 15) / 16), dim3(256), 0, stream,
+                           p.parts, (long)p.nparts, (long)p.width, (int)taps,
+                           dw.data_ptr<float>(), rest.data_ptr<float>());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+        return {dx, dw, db, dstate, Tensor(), Tensor()};
+    }
+};
+
+void check_conv(const char* op, const Tensor& x, const Tensor& w, const OptTensor& bias)
+{
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) >= 2 && w.size(1) <= 4, op,
+                      ": weight must be (channels, taps) with 2 to 4 taps, got ", w.sizes());
+    check_like(op, "weight", w, x, torch::kFloat32, {x.size(-1), w.size(1)});
+    if (bias) check_like(op, "bias", *bias, x, torch::kFloat32, {x.size(-1)});
+}
+
+bool wants_grad(std::initializer_list<OptTensor> all)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (auto& t : all)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+
+Tensor dense(const Tensor& t) { return t.contiguous(); }
+OptTensor dense(const OptTensor& t) { return t ? c10::make_optional(t->contiguous()) : t; }
+
+std::vector<Tensor> causal_conv(const Tensor& x_in, const Tensor& w, const OptTensor& bias,
+                                const OptTensor& state, const OptTensor& mask, bool silu)
+{
+    const char* op = "causal_conv";
+    check_x(op, x_in, 3);
+    check_conv(op, x_in, w, bias);
+    if (state)
+        check_like(op, "state", *state, x_in, x_in.scalar_type(),
+                   {x_in.size(0), w.size(1) - 1, x_in.size(2)});
+    const auto x = dense_last(x_in);
+    const auto m = as_mask(op, mask, x);
+    if (wants_grad({x, w, bias, state}))
+        return CausalConv::apply(x, dense(w), dense(bias), dense(state),
+                                 m.defined() ? OptTensor(m) : OptTensor(), silu);
+    return conv_forward(x, w.contiguous(), dense(bias).value_or(Tensor()),
+                        dense(state).value_or(Tensor()), m, silu);
+}
+
+Tensor causal_conv_step(Tensor state, const Tensor& x_in, const Tensor& w, const OptTensor& bias,
+                        const OptTensor& mask, bool silu)
+{
+    const char* op = "causal_conv_step";
+    check_x(op, x_in, 2);
+    check_conv(op, x_in, w, bias);
+    check_like(op, "state", state, x_in, x_in.scalar_type(),
+               {x_in.size(0), w.size(1) - 1, x_in.size(1)});
+    TORCH_CHECK_VALUE(state.is_contiguous(), op, ": state must be contiguous");
+    TORCH_CHECK_VALUE(!wants_grad({x_in, w, bias, state}), op,
+                      ": has no gradient; use causal_conv over one step");
+    const auto x = dense_last(x_in);
+    const auto m = as_mask(op, mask, x);
+    const c10::DeviceGuard guard(x.device());
+    auto y = torch::empty(x.sizes(), x.options());
+    if (x.size(0) == 0) return y;
+    const auto wc = w.contiguous(), bc = dense(bias).value_or(Tensor());
+    ConvArgs p = conv_args(x, wc, bc, Tensor(), m, silu);
+    p.y = y.data_ptr(); p.last = state.data_ptr();
+    by_conv(x, w.size(1), conv_wide(x, {state}),
+            [&](auto t, auto k, auto v) {
+        const int64_t n = blocks_for(p.batch * (p.width / v.value), op);
+        hipLaunchKernelGGL((conv_step_kernel<decltype(t), decltype(k)::value,
+                            decltype(v)::value>), dim3(n), dim3(256), 0,
+                           at::cuda::getCurrentCUDAStream(), p);
+    });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    moved_on(state);
+    return y;
+}
+
+// ---- scan
+
+int lanes_for(int64_t states)
+{
+    int l = 1;
+    while (4 * l < states) l *= 2;
+    return l;
+}
+template <typename F> void by_lanes(int l, F f)
+{
+    if (l == 1) f(Const<1>());
+    else if (l == 2) f(Const<2>());
+    else if (l == 4) f(Const<4>());
+    else if (l == 8) f(Const<8>());
+    else f(Const<16>());
+}
+template <typename F> void by_scan(const Tensor& x, int l, F f)
+{
+    by_type(x, [&](auto t) { by_lanes(l, [&](auto n) { f(t, n); }); });
+}
+
+struct ScanIn {
+    Tensor x, dt, A, B, C, D, z, bias, state, mask;
+    bool softplus;
+};
+
+ScanArgs scan_args(const ScanIn& s)
+{
+    ScanArgs p{};
+    p.x = ptr(s.x); p.dt = ptr(s.dt); p.z = ptr(s.z); p.B = ptr(s.B); p.C = ptr(s.C);
+    p.A = fptr(s.A); p.D = fptr(s.D); p.bias = fptr(s.bias); p.state = fptr(s.state);
+    p.mask = mptr(s.mask);
+    p.batch = s.x.size(0); p.steps = s.x.size(1); p.chunks = (p.steps + TC - 1) / TC;
+    p.xb = s.x.stride(0); p.xt = s.x.stride(1);
+    p.db = s.dt.stride(0); p.dt_ = s.dt.stride(1);
+    if (s.z.defined()) { p.zb = s.z.stride(0); p.zt = s.z.stride(1); }
+    p.Bb = s.B.stride(0); p.Bt = s.B.stride(1); p.Bg = s.B.stride(2);
+    p.Cb = s.C.stride(0); p.Ct = s.C.stride(1); p.Cg = s.C.stride(2);
+    p.width = (int)s.x.size(2); p.states = (int)s.A.size(1); p.groups = (int)s.B.size(2);
+    p.per = p.width / p.groups;
+    const int cb = 256 / lanes_for(p.states);
+    p.tiles = (p.per + cb - 1) / cb;
+    p.segs = 1;
+    p.seg_chunks = (int)p.chunks;
+    p.softplus = s.softplus;
+    p.vec_d = p.per % 4 == 0 && aligned(s.x, 4) && aligned(s.dt, 4) &&
+              (!s.z.defined() || aligned(s.z, 4));
+    p.vec_n = p.states % 4 == 0 && aligned(s.A, 4) && (!s.state.defined() || aligned(s.state, 4));
+    p.vec_b = aligned(s.B, 4) && aligned(s.C, 4);
+    return p;
+}
+
+int64_t scan_blocks(const ScanArgs& p)
+{
+    const int64_t n = p.batch * p.segs * p.groups * p.tiles;
+    TORCH_CHECK_VALUE(n < (1LL << 31), "selective_scan: too large for one launch");
+    return n;
+}
+
+// y, last state and, to train, the state before each chunk
+std::vector<Tensor> scan_forward(const ScanIn& s, bool train)
+{
+    const c10::DeviceGuard guard(s.x.device());
+    auto stream = at::cuda::getCurrentCUDAStream();
+    ScanArgs p = scan_args(s);
+    auto fp32 = s.A.options();
+    auto y = torch::empty(s.x.sizes(), s.x.options());
+    auto last = torch::empty({p.batch, p.width, p.states}, fp32);
+    auto ckpt = train ? torch::empty({p.batch, p.chunks, p.width, p.states}, fp32) : Tensor();
+    if (p.batch == 0 || p.steps == 0) {
+        if (s.state.defined()) last.copy_(s.state); else last.zero_();
+        return {y, last, ckpt};
+    }
+    p.y = y.data_ptr(); p.last = last.data_ptr<float>();
+    p.ckpt = train ? ckpt.data_ptr<float>() : nullptr;
+    const int l = lanes_for(p.states);
+    by_scan(s.x, l, [&](auto t, auto n) {
+        hipLaunchKernelGGL((scan_fwd_kernel<decltype(t), decltype(n)::value, false>),
+                           dim3(scan_blocks(p)), dim3(256), 0, stream, p);
+    });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    return {y, last, ckpt};
+}
+
+class SelectiveScan : public torch::autograd::Function<SelectiveScan> {
+public:
+    static torch::autograd::variable_list forward(
+        torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& dt, const Tensor& A,
+        const Tensor& B, const Tensor& C, const OptTensor& D, const OptTensor& z,
+        const OptTensor& bias, const OptTensor& state, const OptTensor& mask, bool softplus)
+    {
+        const Tensor none;
+        ScanIn s{x, dt, A, B, C, D.value_or(none), z.value_or(none), bias.value_or(none),
+                 state.value_or(none), mask.value_or(none), softplus};
+        auto out = scan_forward(s, true);
+        ctx->save_for_backward({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.state, s.mask,
+                                out[2]});
+        ctx->saved_data["softplus"] = softplus;
+        return {out[0], out[1]};
+    }
+
+    static torch::autograd::variable_list backward(
+        torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        TORCH_CHECK(!at::GradMode::is_enabled(),
+                    "selective_scan: its gradients are not differentiable again");
+        auto v = ctx->get_saved_variables();
+        ScanIn s{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9],
+                 ctx->saved_data["softplus"].toBool()};
+        const auto& ckpt = v[10];
+        const c10::DeviceGuard guard(s.x.device());
+        auto stream = at::cuda::getCurrentCUDAStream();
+        ScanArgs p = scan_args(s);
+        auto fp32 = s.A.options();
+        auto like = [](const Tensor& t) { return torch::empty(t.sizes(), t.options()); };
+        auto dy = grads[0].defined() ? grads[0].contiguous()
+                                     : torch::zeros(s.x.sizes(), s.x.options());
+        auto dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        auto dx = like(s.x), ddt = like(s.dt), dA = like(s.A), dB = like(s.B), dC = like(s.C);
+        auto dD = torch::empty({2, p.width}, fp32);
+        auto dz = s.z.defined() ? like(s.z) : Tensor();
+        auto dstate = s.state.defined() ? like(s.state) : Tensor();
+        torch::autograd::variable_list out(11);
+        out[0] = dx; out[1] = ddt; out[2] = dA; out[3] = dB; out[4] = dC;
+        if (s.D.defined()) out[5] = dD[0];
+        out[6] = dz;
+        if (s.bias.defined()) out[7] = dD[1];
+        out[8] = dstate;
+        if (p.batch == 0 || p.steps == 0) {
+            dA.zero_(); dD.zero_();
+            if (dstate.defined()) {
+                if (dlast.defined()) dstate.copy_(dlast); else dstate.zero_();
+            }
+            return out;
+        }
+        const int64_t rows = p.batch * p.segs, nb = dB.numel();
+        auto bc = torch::empty({2, p.tiles, nb}, fp32);
+        auto dAp = torch::empty({rows, p.width, p.states}, fp32);
+        auto dDp = torch::empty({rows, 2, p.width}, fp32);
+        p.dy = ptr(dy); p.dlast = fptr(dlast);
+        p.vec_d = p.vec_d && aligned(dy, 4);
+        p.vec_n = p.vec_n && (!dlast.defined() || aligned(dlast, 4));
+        p.ckpt = ckpt.data_ptr<float>();
+        p.dx = dx.data_ptr(); p.ddt = ddt.data_ptr(); p.dz = dz.defined() ? dz.data_ptr() : nullptr;
+        p.dBp = bc.data_ptr<float>(); p.dCp = p.dBp + p.tiles * nb;
+        p.dAp = dAp.data_ptr<float>(); p.dDp = dDp.data_ptr<float>();
+        p.dstate = dstate.defined() ? dstate.data_ptr<float>() : nullptr;
+        by_scan(s.x, lanes_for(p.states), [&](auto t, auto n) {
+            using T = decltype(t);
+            hipLaunchKernelGGL((scan_bwd_kernel<T, decltype(n)::value, false>),
+                               dim3(scan_blocks(p)), dim3(256), 0, stream, p);
+            const int64_t blocks = blocks_for(nb, "selective_scan");
+            hipLaunchKernelGGL(tile_sum_kernel<T>, dim3(blocks), dim3(256), 0, stream,
+                               p.dBp, p.tiles, (long)nb, (T*)dB.data_ptr());
+            hipLaunchKernelGGL(tile_sum_kernel<T>, dim3(blocks), dim3(256), 0, stream,
+                               p.dCp, p.tiles, (long)nb, (T*)dC.data_ptr());
+        });
+        auto sum = [&](const float* parts, int64_t width, float* to) {
+            hipLaunchKernelGGL(column_sum_kernel, dim3((width + 15) / 16), dim3(256), 0, stream,
+                               parts, (long)rows, (long)width, 1, to, (float*)nullptr);
+        };
+        sum(p.dAp, (int64_t)p.width * p.states, dA.data_ptr<float>());
+        sum(p.dDp, 2 * (int64_t)p.width, dD.data_ptr<float>());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+        return out;
+    }
+};
+
+void check_scan(const char* op, const Tensor& x, const Tensor& dt, const Tensor& A,
+                const Tensor& B, const Tensor& C, const OptTensor& D, const OptTensor& z,
+                const OptTensor& bias)
+{
+    const auto type = x.scalar_type();
+    check_like(op, "dt", dt, x, type, x.sizes());
+    TORCH_CHECK_VALUE(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, op,
+                      ": A must be (channels, states) with 1 to 64 states, got ", A.sizes());
+    check_like(op, "A", A, x, torch::kFloat32, {x.size(-1), A.size(1)});
+    auto shape = x.sizes().slice(0, x.dim() - 1).vec();
+    TORCH_CHECK_VALUE(B.dim() == x.dim() + 1 && B.size(-2) >= 1 &&
+                      x.size(-1) % B.size(-2) == 0, op,
+                      ": B must be (..., groups, states) with groups that divide the channels, got ",
+                      B.sizes());
+    shape.push_back(B.size(-2));
+    shape.push_back(A.size(1));
+    check_like(op, "B", B, x, type, shape);
+    check_like(op, "C", C, x, type, shape);
+    if (D) check_like(op, "D", *D, x, torch::kFloat32, {x.size(-1)});
+    if (z) check_like(op, "z", *z, x, type, x.sizes());
+    if (bias) check_like(op, "dt_bias", *bias, x, torch::kFloat32, {x.size(-1)});
+}
+
+std::vector<Tensor> selective_scan(
+    const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+    const OptTensor& D, const OptTensor& z, const OptTensor& bias, bool softplus,
+    const OptTensor& state, const OptTensor& mask)
+{
+    const char* op = "selective_scan";
+    check_x(op, x, 3);
+    check_scan(op, x, dt, A, B, C, D, z, bias);
+    if (state)
+        check_like(op, "state", *state, x, torch::kFloat32, {x.size(0), x.size(2), A.size(1)});
+    const auto m = as_mask(op, mask, x);
+    const Tensor none;
+    const auto zd = z ? OptTensor(dense_last(*z)) : z;
+    ScanIn s{dense_last(x), dense_last(dt), dense(A), dense_last(B), dense_last(C),
+             dense(D).value_or(none), zd.value_or(none), dense(bias).value_or(none),
+             dense(state).value_or(none), m, softplus};
+    if (wants_grad({x, dt, A, B, C, D, z, bias, state}))
+        return SelectiveScan::apply(s.x, s.dt, s.A, s.B, s.C, dense(D), zd, dense(bias),
+                                    dense(state), m.defined() ? OptTensor(m) : OptTensor(),
+                                    softplus);
+    auto out = scan_forward(s, false);
+    return {out[0], out[1]};
+}
+
+Tensor selective_step(Tensor state, const Tensor& x_in, const Tensor& dt_in, const Tensor& A_in,
+                      const Tensor& B_in, const Tensor& C_in, const OptTensor& D_in,
+                      const OptTensor& z_in, const OptTensor& bias_in, bool softplus,
+                      const OptTensor& mask)
+{
+    const char* op = "selective_step";
+    check_x(op, x_in, 2);
+    check_scan(op, x_in, dt_in, A_in, B_in, C_in, D_in, z_in, bias_in);
+    check_like(op, "state", state, x_in, torch::kFloat32,
+               {x_in.size(0), x_in.size(1), A_in.size(1)});
+    TORCH_CHECK_VALUE(state.is_contiguous(), op, ": state must be contiguous");
+    TORCH_CHECK_VALUE(!wants_grad({x_in, dt_in, A_in, B_in, C_in, D_in, z_in, bias_in, state}),
+                      op, ": has no gradient; use selective_scan over one step");
+    const auto m = as_mask(op, mask, x_in);
+    const c10::DeviceGuard guard(x_in.device());
+    auto y = torch::empty(x_in.sizes(), x_in.options());
+    if (x_in.size(0) == 0) return y;
+    const Tensor none;
+    const auto x = dense_last(x_in), dt = dense_last(dt_in), A = dense(A_in),
+               B = dense_last(B_in), C = dense_last(C_in), D = dense(D_in).value_or(none),
+               z = z_in ? dense_last(*z_in) : none, bias = dense(bias_in).value_or(none);
+    StepArgs p{};
+    p.x = ptr(x); p.dt = ptr(dt); p.z = ptr(z); p.B = ptr(B); p.C = ptr(C);
+    p.A = fptr(A); p.D = fptr(D); p.bias = fptr(bias); p.mask = mptr(m);
+    p.state = state.data_ptr<float>(); p.y = y.data_ptr();
+    p.batch = x.size(0); p.xb = x.stride(0); p.db = dt.stride(0);
+    p.zb = z.defined() ? z.stride(0) : 0;
+    p.Bb = B.stride(0); p.Bg = B.stride(1); p.Cb = C.stride(0); p.Cg = C.stride(1);
+    p.width = (int)x.size(1); p.states = (int)A.size(1); p.groups = (int)B.size(1);
+    p.per = p.width / p.groups; p.softplus = softplus;
+    p.vec_n = p.states % 4 == 0 && aligned(state, 4) && aligned(A, 4);
+    p.vec_b = aligned(B, 4) && aligned(C, 4);
+    const int l = lanes_for(p.states);
+    const int64_t n = blocks_for(p.batch * p.width * l, op);
+    by_scan(x, l, [&](auto t, auto k) {
+        hipLaunchKernelGGL((scan_step_kernel<decltype(t), decltype(k)::value>), dim3(n),
+                           dim3(256), 0, at::cuda::getCurrentCUDAStream(), p);
+    });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    moved_on(state);
+    return y;
+}
+
+}  // namespace
+
+void bind_selective(pybind11::module& m)
+{
+    m.def("causal_conv", &causal_conv, "short causal convolution over a window (y, last state)");
+    m.def("causal_conv_step", &causal_conv_step, "one step of it, the state in place");
+    m.def("selective_scan", &selective_scan, "selective state space scan (y, last state)");
+    m.def("selective_step", &selective_step, "one step of it, the state in place");
+}
