@@ -37,7 +37,7 @@ except ImportError:       # pragma: no cover - psutil is in the image
 from .environment import prepare_env, make_env
 from .util import map_r, bimap_r, trimap_r
 from .model import to_gpu, ModelWrapper
-from .losses import compute_target
+from .losses import POLICY_LOSS_STATS, clipped_policy_loss, compute_target
 from .batch import EpisodeBuffer, Batcher
 from .worker import WorkerCluster, WorkerServer
 from . import dist as hdist
@@ -59,6 +59,8 @@ def forward_prediction(model, hidden, batch, args):
         obs = map_r(observations, lambda o: o.flatten(0, 2))
         outputs = model(obs, None)
         outputs = map_r(outputs, lambda o: o.unflatten(0, batch_shape))
+    elif hasattr(getattr(model, 'model', model), 'forward_window'):
+        outputs = _window_prediction(model, hidden, observations, batch, args)
     else:
         outputs = {}
         for t in range(batch_shape[1]):
@@ -99,6 +101,32 @@ def forward_prediction(model, hidden, batch, args):
     return outputs
 
 
+def _window_prediction(model, hidden, observations, batch, args):
+    """The recurrent outputs of a (B, T, P) batch from nets that take whole
+    windows: ``forward_window(obs, hidden, mask)`` on one row per (episode,
+    seat), each stepping where its seat observes, is called once for the
+    burn-in and once for the training window instead of once per step."""
+    omask = batch['observation_mask']                   # (B, T, P, 1)
+    B, T, P = omask.size()[:3]
+    window = getattr(model, 'model', model).forward_window
+    rows = map_r(observations, lambda o: o.expand(-1, -1, P, *[-1] * (o.dim() - 3))
+                 .transpose(1, 2).flatten(0, 1))
+    mask = omask.view(B, T, P).transpose(1, 2).flatten(0, 1) != 0
+    hidden = map_r(hidden, lambda h: h.flatten(0, 1))
+    cut, parts = args['burn_in_steps'], []
+    if cut > 0:
+        model.eval()
+        with torch.no_grad():
+            parts.append(window(map_r(rows, lambda o: o[:, :cut]), hidden, mask[:, :cut]))
+        hidden = parts[0]['hidden']
+    if not model.training:
+        model.train()
+    parts.append(window(map_r(rows, lambda o: o[:, cut:]), hidden, mask[:, cut:]))
+    keys = [k for k, o in parts[-1].items() if k != 'hidden' and o is not None]
+    return {k: torch.cat([part[k] for part in parts], 1).unflatten(0, (B, P)).transpose(1, 2)
+            for k in keys}
+
+
 def compose_losses(outputs, log_selected_policies, total_advantages, targets, batch, args):
     """Summed (not averaged) loss terms + the data count that scales lr."""
     tmasks = batch['turn_mask']
@@ -125,6 +153,32 @@ def compose_losses(outputs, log_selected_policies, total_advantages, targets, ba
     decay = 1 - batch['progress'] * (1 - args['entropy_regularization_decay'])
     entropy_loss = entropy.mul(decay).sum() * -args['entropy_regularization']
     losses['total'] = base_loss + entropy_loss
+    return losses, dcnt
+
+
+def compose_clipped_losses(outputs, log_behavior, advantages, targets, batch, args):
+    """compose_losses with the clipped policy loss and its KL term
+    (losses.clipped_policy_loss) for ``policy_loss: 'CLIP'``."""
+    tmasks, omasks = batch['turn_mask'], batch['observation_mask']
+    policy = outputs['policy']
+    dcnt = tmasks.sum()
+    if policy.size(2) != tmasks.size(2):        # one seat acts: take its advantage
+        advantages = (advantages * tmasks).sum(2, keepdim=True)
+        tmasks = tmasks.sum(2, keepdim=True)
+    decay = 1 - batch['progress'] * (1 - args['entropy_regularization_decay'])
+    total, sums = clipped_policy_loss(
+        policy, batch['action'], log_behavior, advantages.detach(), tmasks, decay,
+        clip=args.get('clip_ratio', 0.2), kl_coef=args.get('kl_regularization', 0.0),
+        entropy_coef=args['entropy_regularization'])
+    sums = dict(zip(POLICY_LOSS_STATS, sums.unbind()))
+    losses = {'p': sums['p']}
+    if 'value' in outputs:
+        losses['v'] = ((outputs['value'] - targets['value']) ** 2).mul(omasks).sum() / 2
+    if 'return' in outputs:
+        losses['r'] = F.smooth_l1_loss(outputs['return'], targets['return'],
+                                       reduction='none').mul(omasks).sum()
+    losses.update(kl=sums['kl'], clip=sums['clipped'], ent=sums['ent'])
+    losses['total'] = total + losses.get('v', 0) + losses.get('r', 0)
     return losses, dcnt
 
 
@@ -183,7 +237,8 @@ def _fused_loss_ok(outputs, batch, args):
             and 'value' in outputs and 'return' not in outputs
             and outputs['policy'].dim() == 4
             and outputs['policy'].size(2) == 1       # solo seat axis
-            and not args['turn_based_training'])
+            and not args['turn_based_training']
+            and args.get('policy_loss', 'PG') == 'PG')
 
 
 def _compute_loss_fused(outputs, batch, args):
@@ -210,6 +265,9 @@ def _compute_loss_fused(outputs, batch, args):
 
 
 def compute_loss(batch, model, hidden, args):
+    policy_loss = args.get('policy_loss', 'PG')
+    if policy_loss not in ('PG', 'CLIP'):
+        raise ValueError('unknown policy_loss %r' % (policy_loss,))
     outputs = forward_prediction(model, hidden, batch, args)
     if args['burn_in_steps'] > 0:
         batch = map_r(batch, lambda v: v[:, args['burn_in_steps']:] if v.size(1) > 1 else v)
@@ -264,6 +322,10 @@ def compute_loss(batch, model, hidden, args):
     if args['policy_target'] != args['value_target']:
         _, advantages['value'] = compute_target(args['policy_target'], *value_args)
         _, advantages['return'] = compute_target(args['policy_target'], *return_args)
+
+    if policy_loss == 'CLIP':       # the ratio stands in the loss itself
+        return compose_clipped_losses(outputs, log_selected_b_policies,
+                                      sum(advantages.values()), targets, batch, args)
 
     total_advantages = clipped_rhos * sum(advantages.values())
     return compose_losses(outputs, log_selected_t_policies, total_advantages,
