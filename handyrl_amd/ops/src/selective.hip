@@ -376,6 +376,45 @@ template <int L> __device__ __forceinline__ float channel_sum(float v) {
     return v;
 }
 
+// Adds a to b across the halves of a wave (32) or across neighbouring rows of
+// 16 lanes (16): the first lanes of each pair get a's sum, the others b's.
+__device__ __forceinline__ float fold32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(
+        __builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned lo = r[0], hi = r[1];    // a bit_cast of r[1] itself reads r[0]
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(
+        __builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned lo = r[0], hi = r[1];    // a bit_cast of r[1] itself reads r[0]
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// Sums eight values over a wave's channels (lanes L apart), halving the number
+// of values with each exchange: 16 instructions for L = 4 instead of 8 x 4
+// exchanges and sums.  The sum of vb[i] is then in the lanes with bit 5 of i's
+// bit 0 and bit 4 of its bit 1, that of vc[i] in those with bit 3 set too (for
+// L = 16: in the second value).
+template <int L>
+__device__ __forceinline__ void wave_fold(const float (&vb)[4], const float (&vc)[4],
+                                          float& first, float& second) {
+    const float b = fold16(fold32(vb[0], vb[1]), fold32(vb[2], vb[3]));
+    const float c = fold16(fold32(vc[0], vc[1]), fold32(vc[2], vc[3]));
+    if (L == 16) {
+        first = b;
+        second = c;
+        return;
+    }
+    const bool upper = threadIdx.x & 8;
+    float v = upper ? c : b, w = upper ? b : c;
+    v += dpp<0x128>(w);                 // the row turned by 8
+    if (L < 8) v += dpp<0x104>(v);      // from 4 lanes above
+    if (L < 4) v += dpp<0x4E>(v);
+    if (L < 2) v += dpp<0xB1>(v);
+    first = second = v;
+}
+
 // Which rows, channels and steps a block has: 256 threads take 256/L channels
 // of one group, L lanes a channel and four states a lane.
 template <int L> struct Place {
@@ -416,7 +455,7 @@ template <int L> struct Part {
     }
 };
 
-template <typename T, int L>
+template <typename T, int L, bool WANT_B = true, bool WANT_C = true>
 __device__ __forceinline__ void stage_bc(const ScanArgs& p, const Place<L>& at, long t0,
                                          float (*sB)[4 * L], float (*sC)[4 * L]) {
     const int tid = threadIdx.x;
@@ -425,19 +464,23 @@ __device__ __forceinline__ void stage_bc(const ScanArgs& p, const Place<L>& at, 
         float vb[4] = {}, vc[4] = {};
         const long s = t0 + t;
         if (s < p.steps && (!p.mask || p.mask[at.b * p.steps + s])) {
-            load4((const T*)p.B + at.b * p.Bb + s * p.Bt + at.g * p.Bg + n, p.states - n, p.vec_b, vb);
-            load4((const T*)p.C + at.b * p.Cb + s * p.Ct + at.g * p.Cg + n, p.states - n, p.vec_b, vc);
+            if (WANT_B)
+                load4((const T*)p.B + at.b * p.Bb + s * p.Bt + at.g * p.Bg + n, p.states - n,
+                      p.vec_b, vb);
+            if (WANT_C)
+                load4((const T*)p.C + at.b * p.Cb + s * p.Ct + at.g * p.Cg + n, p.states - n,
+                      p.vec_b, vc);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            sB[t][n + i] = vb[i];
-            sC[t][n + i] = vc[i];
+            if (WANT_B) sB[t][n + i] = vb[i];
+            if (WANT_C) sC[t][n + i] = vc[i];
         }
     }
 }
 
 // x and d = softplus(dt + bias) of a thread's part; zeros where nothing is.
-template <typename T, int L>
+template <typename T, int L, bool WANT_X = true>
 __device__ __forceinline__ bool load_xd(const ScanArgs& p, const Place<L>& at, const Part<L>& q,
                                         long t0, float* x, float* d, float* raw) {
     const long s = t0 + q.t;
@@ -447,7 +490,7 @@ __device__ __forceinline__ bool load_xd(const ScanArgs& p, const Place<L>& at, c
     for (int i = 0; i < 4; ++i) x[i] = d[i] = raw[i] = 0.f;
     if (on) {
         const int c = at.c0 + q.c;
-        load4((const T*)p.x + at.b * p.xb + s * p.xt + c, n, p.vec_d, x);
+        if (WANT_X) load4((const T*)p.x + at.b * p.xb + s * p.xt + c, n, p.vec_d, x);
         load4((const T*)p.dt + at.b * p.db + s * p.dt_ + c, n, p.vec_d, raw);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -473,6 +516,7 @@ template <typename T, int L, bool LOCAL>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
 {
     const Place<L> at(p);
+    if (LOCAL && at.seg == p.segs - 1) return;          // nothing lies behind it
     __shared__ float2 sdu[TC][256 / L];
     __shared__ float sB[TC][4 * L], sC[TC][4 * L], sy[TC][256 / L];
 
@@ -504,7 +548,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sdu[q.t][q.c + i] = make_float2(d[i], d[i] * x[j][i]);
         }
-        stage_bc<T, L>(p, at, t0, sB, sC);
+        stage_bc<T, L, true, !LOCAL>(p, at, t0, sB, sC);
         __syncthreads();
         if (!LOCAL && p.ckpt && at.nn > 0)
             store4(p.ckpt + at.state_at(p, at.b * p.chunks + k), at.nn, p.vec_n, h);
@@ -569,11 +613,12 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs p)
 {
     constexpr int CB = 256 / L, NP = 4 * L;
     const Place<L> at(p);
+    if (LOCAL && at.seg == 0) return;                   // nothing lies before it
     __shared__ float2 sdx[TC][CB];                      // d, x
     __shared__ float sg[TC][CB], sB[TC][NP], sC[TC][NP];
     __shared__ float2 ss[LOCAL ? 1 : TC][CB];           // sum lam B, sum A2 a h lam
     __shared__ float sy[LOCAL ? 1 : TC][CB];
-    __shared__ float2 sbc[LOCAL ? 1 : 4][TC][NP];       // each wave's dB, dC
+    __shared__ float sbc[LOCAL ? 1 : 4][TC][2][NP];     // each wave's dB, dC
 
     float A2[4], lam[4] = {}, dA[4] = {}, total = 0.f;
     float dD[4] = {}, dbias[4] = {};
@@ -600,7 +645,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs p)
         for (int j = 0; j < NQ; ++j) {
             const Part<L> q(j);
             float d[4];
-            on[j] = load_xd<T, L>(p, at, q, t0, x[j], d, raw[j]);
+            on[j] = load_xd<T, L, !LOCAL>(p, at, q, t0, x[j], d, raw[j]);
             const int c = at.c0 + q.c, n = at.nc - q.c;
             const long s = t0 + q.t;
 #pragma unroll
@@ -616,7 +661,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs p)
                     sg[q.t][q.c + i] = p.z ? dy[j][i] * z[j][i] * sigmoid(z[j][i]) : dy[j][i];
                 }
         }
-        stage_bc<T, L>(p, at, t0, sB, sC);
+        stage_bc<T, L, !LOCAL, true>(p, at, t0, sB, sC);
         __syncthreads();
 
         if (LOCAL) {
@@ -671,18 +716,16 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs p)
                 s1 = channel_sum<L>(s1);
                 s2 = channel_sum<L>(s2);
                 if (at.n0 == 0) ss[t][at.c] = make_float2(s1, s2);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int o = L; o < 64; o <<= 1) {
-                        vb[i] += __shfl_xor(vb[i], o);
-                        vc[i] += __shfl_xor(vc[i], o);
-                    }
+                float b, c;
+                wave_fold<L>(vb, vc, b, c);
+                const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+                const int n = at.n0 + (lane >> 5) + 2 * ((lane >> 4) & 1);
+                if (L == 16) {
+                    sbc[wave][t][0][n] = b;
+                    sbc[wave][t][1][n] = c;
+                } else if ((lane & 7) < L) {
+                    sbc[wave][t][(lane >> 3) & 1][n] = b;
                 }
-                if ((threadIdx.x & 63) < L)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sbc[threadIdx.x >> 6][t][at.n0 + i] = make_float2(vb[i], vc[i]);
             }
             __syncthreads();
 #pragma unroll
@@ -723,8 +766,8 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs p)
                 float vb = 0.f, vc = 0.f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    vb += sbc[w][t][n].x;
-                    vc += sbc[w][t][n].y;
+                    vb += sbc[w][t][0][n];
+                    vc += sbc[w][t][1][n];
                 }
                 p.dBp[to] = vb;
                 p.dCp[to] = vc;
@@ -1121,6 +1164,20 @@ struct ScanIn {
     bool softplus;
 };
 
+// Cuts the steps into segments that run side by side where rows and channels
+// alone leave the card idle; their states are joined by one more pass.
+void cut_steps(ScanArgs& p)
+{
+    // 1024 blocks are four waves a SIMD.  1x8192x1024 forward: 2410 us in one
+    // piece, 249 with 256 blocks, 112 with 1024 and 111 with 2048 or 4096;
+    // 4x2048x2048 backward: 1444 us in one piece, 937 with 1024, 1034 with 4096.
+    const int64_t target = 1024;
+    const int64_t blocks = std::max<int64_t>(1, p.batch * p.groups * p.tiles);
+    int64_t segs = std::max<int64_t>(1, std::min({target / blocks, p.chunks, (int64_t)64}));
+    p.seg_chunks = (int)std::max<int64_t>(1, (p.chunks + segs - 1) / segs);
+    p.segs = (int)std::max<int64_t>(1, (p.chunks + p.seg_chunks - 1) / p.seg_chunks);
+}
+
 ScanArgs scan_args(const ScanIn& s)
 {
     ScanArgs p{};
@@ -1137,8 +1194,7 @@ ScanArgs scan_args(const ScanIn& s)
     p.per = p.width / p.groups;
     const int cb = 256 / lanes_for(p.states);
     p.tiles = (p.per + cb - 1) / cb;
-    p.segs = 1;
-    p.seg_chunks = (int)p.chunks;
+    cut_steps(p);
     p.softplus = s.softplus;
     p.vec_d = p.per % 4 == 0 && aligned(s.x, 4) && aligned(s.dt, 4) &&
               (!s.z.defined() || aligned(s.z, 4));
@@ -1152,6 +1208,17 @@ int64_t scan_blocks(const ScanArgs& p)
     const int64_t n = p.batch * p.segs * p.groups * p.tiles;
     TORCH_CHECK_VALUE(n < (1LL << 31), "selective_scan: too large for one launch");
     return n;
+}
+
+// What the segments hand on: a state and the sum of their steps.
+Tensor segment_buffers(ScanArgs& p, const torch::TensorOptions& fp32)
+{
+    if (p.segs == 1) return Tensor();
+    const int64_t rows = p.batch * p.segs * p.width;
+    auto t = torch::empty({rows * (p.states + 1)}, fp32);
+    p.seg_h = t.data_ptr<float>();
+    p.seg_d = p.seg_h + rows * p.states;
+    return t;
 }
 
 // y, last state and, to train, the state before each chunk
@@ -1170,8 +1237,11 @@ std::vector<Tensor> scan_forward(const ScanIn& s, bool train)
     }
     p.y = y.data_ptr(); p.last = last.data_ptr<float>();
     p.ckpt = train ? ckpt.data_ptr<float>() : nullptr;
-    const int l = lanes_for(p.states);
-    by_scan(s.x, l, [&](auto t, auto n) {
+    const auto seg = segment_buffers(p, fp32);
+    by_scan(s.x, lanes_for(p.states), [&](auto t, auto n) {
+        if (p.segs > 1)
+            hipLaunchKernelGGL((scan_fwd_kernel<decltype(t), decltype(n)::value, true>),
+                               dim3(scan_blocks(p)), dim3(256), 0, stream, p);
         hipLaunchKernelGGL((scan_fwd_kernel<decltype(t), decltype(n)::value, false>),
                            dim3(scan_blocks(p)), dim3(256), 0, stream, p);
     });
@@ -1242,8 +1312,12 @@ public:
         p.dBp = bc.data_ptr<float>(); p.dCp = p.dBp + p.tiles * nb;
         p.dAp = dAp.data_ptr<float>(); p.dDp = dDp.data_ptr<float>();
         p.dstate = dstate.defined() ? dstate.data_ptr<float>() : nullptr;
+        const auto seg = segment_buffers(p, fp32);
         by_scan(s.x, lanes_for(p.states), [&](auto t, auto n) {
             using T = decltype(t);
+            if (p.segs > 1)
+                hipLaunchKernelGGL((scan_bwd_kernel<T, decltype(n)::value, true>),
+                                   dim3(scan_blocks(p)), dim3(256), 0, stream, p);
             hipLaunchKernelGGL((scan_bwd_kernel<T, decltype(n)::value, false>),
                                dim3(scan_blocks(p)), dim3(256), 0, stream, p);
             const int64_t blocks = blocks_for(nb, "selective_scan");
