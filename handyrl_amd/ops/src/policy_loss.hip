@@ -546,6 +546,7 @@ public:
         ctx->saved_data["capture"] = (int64_t)capture_of(
             at::cuda::getCurrentCUDAStream(logits.device().index()));
         ctx->mark_non_differentiable({out[1]});
+        ctx->set_materialize_grads(false);
         return {out[0], out[1]};
     }
 
@@ -554,6 +555,8 @@ public:
     {
         TORCH_CHECK(!at::GradMode::is_enabled(),
                     "clipped_policy_loss: its gradient is not differentiable again");
+        torch::autograd::variable_list out(10);
+        if (!grads[0].defined()) return out;
         auto saved = ctx->get_saved_variables();
         const auto& logits = saved[0];
         const auto coefs = ctx->saved_data["coefs"].toDoubleVector();
@@ -575,7 +578,6 @@ public:
         p.upstream = up.data_ptr<float>();
         p.skip_one = ready;
         launch(logits, p, stream, false);
-        torch::autograd::variable_list out(10);
         out[0] = grad;
         return out;
     }
