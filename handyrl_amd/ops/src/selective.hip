@@ -635,6 +635,22 @@ __device__ __forceinline__ void join_segment(const ScanArgs& p, const Place<L>& 
     for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_fast(A2[i] * d), h[i], e[i]);
 }
 
+// What a lane reads of one step.  The next step's is read before the present one
+// is computed: the compiler alone reads just before the use, and each step then
+// waits for shared memory (4x2048x2048 backward: 347 us against 318).
+struct StepIn {
+    float2 v;
+    float g, B[4], C[4];
+    template <bool HAS_G, bool HAS_B, bool HAS_C>
+    __device__ __forceinline__ void read(const float2* sv, const float* sg, const float* sB,
+                                         const float* sC, int c, int n0) {
+        v = sv[c];
+        if (HAS_G) g = sg[c];
+        if (HAS_B) load_pack<float, 4>(sB + n0, B);
+        if (HAS_C) load_pack<float, 4>(sC + n0, C);
+    }
+};
+
 // LOCAL: the segment's own end from a zero start, and its sum of d, for the
 // segments behind it.  Otherwise the outputs, from the state before the
 // segment: the carried one moved through the segments before.
@@ -680,19 +696,24 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
         __syncthreads();
         if (k + 1 < k1) next.template fetch<true, !LOCAL, false, true, !LOCAL>(p, at, t0 + TC);
         // steps behind the end have d = 0 and x = 0 and change nothing
+        StepIn in[2];
+        in[0].template read<false, true, !LOCAL>(sdu[0], nullptr, sB[0], sC[0], at.c, at.n0);
 #pragma unroll
         for (int t = 0; t < TC; ++t) {
             if (!LOCAL && t % TH == 0 && p.ckpt && at.nn > 0)
                 store4(p.ckpt + at.state_at(p, (at.b * p.chunks + k) * (TC / TH) + t / TH), at.nn,
                        p.vec_n, h);
-            const float2 v = sdu[t][at.c];
+            if (t + 1 < TC)
+                in[(t + 1) & 1].template read<false, true, !LOCAL>(
+                    sdu[t + 1], nullptr, sB[t + 1], sC[t + 1], at.c, at.n0);
+            const StepIn& s = in[t & 1];
             float y = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                h[i] = fmaf(exp2_fast(A2[i] * v.x), h[i], v.y * sB[t][at.n0 + i]);
-                if (!LOCAL) y = fmaf(sC[t][at.n0 + i], h[i], y);
+                h[i] = fmaf(exp2_fast(A2[i] * s.v.x), h[i], s.v.y * s.B[i]);
+                if (!LOCAL) y = fmaf(s.C[i], h[i], y);
             }
-            if (LOCAL) total += v.x;
+            if (LOCAL) total += s.v.x;
             else sy[t][at.c] = channel_sum<L>(y);       // the same from all its lanes
         }
         __syncthreads();
@@ -785,13 +806,19 @@ __global__ __launch_bounds__(256, LOCAL ? 4 : 2) void scan_bwd_kernel(ScanArgs p
         if (k > k0) next.template fetch<!LOCAL, true, true, !LOCAL, true>(p, at, t0 - TC);
 
         if (LOCAL) {
+            StepIn in[2];
+            in[1].template read<true, false, true>(sdx[TC - 1], sg[TC - 1], nullptr, sC[TC - 1],
+                                                   at.c, at.n0);
 #pragma unroll
             for (int t = TC - 1; t >= 0; --t) {
-                const float d = sdx[t][at.c].x, g = sg[t][at.c];
-                total += d;
+                if (t > 0)
+                    in[(t - 1) & 1].template read<true, false, true>(sdx[t - 1], sg[t - 1], nullptr,
+                                                                     sC[t - 1], at.c, at.n0);
+                const StepIn& s = in[t & 1];
+                total += s.v.x;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    lam[i] = exp2_fast(A2[i] * d) * fmaf(sC[t][at.n0 + i], g, lam[i]);
+                    lam[i] = exp2_fast(A2[i] * s.v.x) * fmaf(s.C[i], s.g, lam[i]);
             }
             __syncthreads();
             continue;
@@ -811,34 +838,44 @@ __global__ __launch_bounds__(256, LOCAL ? 4 : 2) void scan_bwd_kernel(ScanArgs p
                 const long row = (at.b * p.chunks + k) * (TC / TH) + u / TH - 1;
                 if ((k > k0 || u > 0) && at.nn > 0)
                     load4(p.ckpt + at.state_at(p, row), at.nn, p.vec_n, first);
+                StepIn in[2];
+                in[0].template read<false, true, true>(sdx[u], nullptr, sB[u], sC[u], at.c, at.n0);
 #pragma unroll
                 for (int t = 0; t < TH; ++t) {
-                    const float2 v = sdx[u + t][at.c];
-                    const float du = v.x * v.y;
+                    if (t + 1 < TH)
+                        in[(t + 1) & 1].template read<false, true, true>(
+                            sdx[u + t + 1], nullptr, sB[u + t + 1], sC[u + t + 1], at.c, at.n0);
+                    else
+                        in[t & 1].g = sg[u + t][at.c];  // where the way back begins
+                    const StepIn& s = in[t & 1];
+                    const float du = s.v.x * s.v.y;
                     float y = 0.f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        a[t][i] = exp2_fast(A2[i] * v.x);
-                        hs[t + 1][i] = fmaf(a[t][i], hs[t][i], du * sB[u + t][at.n0 + i]);
-                        y = fmaf(sC[u + t][at.n0 + i], hs[t + 1][i], y);
+                        a[t][i] = exp2_fast(A2[i] * s.v.x);
+                        hs[t + 1][i] = fmaf(a[t][i], hs[t][i], du * s.B[i]);
+                        y = fmaf(s.C[i], hs[t + 1][i], y);
                     }
                     sy[u + t][at.c] = channel_sum<L>(y);        // the same from all its lanes
                 }
 #pragma unroll
                 for (int t = TH - 1; t >= 0; --t) {
-                    const float2 v = sdx[u + t][at.c];
-                    const float du = v.x * v.y, g = sg[u + t][at.c];
+                    if (t > 0)
+                        in[(t - 1) & 1].template read<true, true, true>(
+                            sdx[u + t - 1], sg[u + t - 1], sB[u + t - 1], sC[u + t - 1], at.c, at.n0);
+                    const StepIn& s = in[t & 1];
+                    const float du = s.v.x * s.v.y;
                     float s1 = 0.f, s2 = 0.f, vb[4], vc[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float l = fmaf(sC[u + t][at.n0 + i], g, lam[i]);
-                        vc[i] = g * hs[t + 1][i];
+                        const float l = fmaf(s.C[i], s.g, lam[i]);
+                        vc[i] = s.g * hs[t + 1][i];
                         vb[i] = l * du;
-                        s1 = fmaf(l, sB[u + t][at.n0 + i], s1);
+                        s1 = fmaf(l, s.B[i], s1);
                         lam[i] = a[t][i] * l;
                         const float ah = lam[i] * hs[t][i];
                         s2 = fmaf(A2[i], ah, s2);
-                        dA[i] = fmaf(v.x, ah, dA[i]);
+                        dA[i] = fmaf(s.v.x, ah, dA[i]);
                     }
                     s1 = channel_sum<L>(s1);
                     s2 = channel_sum<L>(s2);
