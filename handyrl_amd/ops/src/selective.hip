@@ -1018,50 +1018,89 @@ struct StepArgs {
     float* state;
     void* y;
     long batch, xb, db, zb, Bb, Bg, Cb, Cg;
-    int width, states, groups, per, softplus, vec_n, vec_b;
+    int width, states, groups, per, rows, softplus, vec_n, vec_b;
 };
 
-// One step: four states a lane, L lanes a channel, the state in place.
+// A state's four values, past the caches where `once` says that they are far
+// more than those hold.
+typedef float float4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Pack<float, 4> load_once(const float* p, int n, bool whole, bool once) {
+    if (!whole || !once) return load_raw(p, n, whole);
+    return __builtin_bit_cast(Pack<float, 4>, __builtin_nontemporal_load((const float4v*)p));
+}
+__device__ __forceinline__ void store_once(float* p, int n, bool whole, bool once,
+                                           const Pack<float, 4>& h) {
+    if (whole && once) __builtin_nontemporal_store(__builtin_bit_cast(float4v, h), (float4v*)p);
+    else store4(p, n, whole, h.v);
+}
+
+constexpr int SR = 2;           // rows that a lane of a large step has in flight
+
+// One step: four states a lane, L lanes a channel, the state in place.  What
+// bounds it is the state's way to the lane and back.  8192 x 512 x 16 with every
+// other row observed (286 MB): 114 us with a row a lane, 102 with two, 85 with
+// the masks read first and the state past the caches (105 with one row); four
+// rows a lane take 91, for their registers take waves.
 template <typename T, int L>
 __global__ __launch_bounds__(256) void scan_step_kernel(StepArgs p)
 {
     const long at = (long)blockIdx.x * 256 + threadIdx.x;
     const int n0 = 4 * (int)(at % L);
-    const long row = at / L;                            // (b, channel)
-    const long b = row / p.width;
-    const int c = (int)(row % p.width), g = c / p.per;
-    const bool in = b < p.batch, on = in && (!p.mask || p.mask[b]);
-    const int nn = on ? min(4, max(0, p.states - n0)) : 0;
-    float y = 0.f, x = 0.f;
-    if (on) {
-        float raw = to_float(((const T*)p.dt)[b * p.db + c]);
-        x = to_float(((const T*)p.x)[b * p.xb + c]);
-        if (p.bias) raw += p.bias[c];
-        const float d = p.softplus ? softplus(raw) : raw, du = d * x;
-        if (nn > 0) {
-            float h[4], A[4], vb[4], vc[4];
-            load4(p.state + row * p.states + n0, nn, p.vec_n, h);
-            load4(p.A + (long)c * p.states + n0, nn, p.vec_n, A);
-            load4((const T*)p.B + b * p.Bb + g * p.Bg + n0, nn, p.vec_b, vb);
-            load4((const T*)p.C + b * p.Cb + g * p.Cg + n0, nn, p.vec_b, vc);
+    const long item = at / L;                           // (rows, channel)
+    const unsigned width = p.width;
+    const long b0 = item / width * p.rows;
+    const int c = (int)(item % width), g = c / p.per;
+    const int have = min(4, p.states - n0);             // none of a lane behind the states
+    Pack<float, 4> h[SR];
+    Pack<T, 4> vb[SR], vc[SR];
+    T x[SR], dt[SR], z[SR];
+    float A[4] = {};
+    bool in[SR], on[SR];
+#pragma unroll
+    for (int u = 0; u < SR; ++u) {
+        in[u] = u < p.rows && b0 + u < p.batch;
+        on[u] = in[u];
+        if (in[u] && p.mask) on[u] = p.mask[b0 + u];
+    }
+#pragma unroll
+    for (int u = 0; u < SR; ++u) {
+        const long b = b0 + u;
+        if (!on[u]) continue;
+        if (have > 0) {
+            h[u] = load_once(p.state + (b * width + c) * p.states + n0, have, p.vec_n, p.rows > 1);
+            vb[u] = load_raw((const T*)p.B + b * p.Bb + g * p.Bg + n0, have, p.vec_b);
+            vc[u] = load_raw((const T*)p.C + b * p.Cb + g * p.Cg + n0, have, p.vec_b);
+        }
+        x[u] = ((const T*)p.x)[b * p.xb + c];
+        dt[u] = ((const T*)p.dt)[b * p.db + c];
+        if (p.z) z[u] = ((const T*)p.z)[b * p.zb + c];
+    }
+    if (have > 0) load4(p.A + (long)c * p.states + n0, have, p.vec_n, A);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A[i] *= kLog2e;
+    const float bias = p.bias ? p.bias[c] : 0.f, D = p.D ? p.D[c] : 0.f;
+#pragma unroll
+    for (int u = 0; u < SR; ++u) {
+        const long row = (b0 + u) * width + c;
+        float y = 0.f;
+        if (on[u] && have > 0) {
+            const float raw = to_float(dt[u]) + bias;
+            const float d = p.softplus ? softplus(raw) : raw, du = d * to_float(x[u]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                h[i] = fmaf(exp2_fast(A[i] * kLog2e * d), h[i], du * vb[i]);
-                y = fmaf(vc[i], h[i], y);
+                h[u].v[i] = fmaf(exp2_fast(A[i] * d), h[u].v[i], du * to_float(vb[u].v[i]));
+                y = fmaf(to_float(vc[u].v[i]), h[u].v[i], y);
             }
-            store4(p.state + row * p.states + n0, nn, p.vec_n, h);
+            store_once(p.state + row * p.states + n0, have, p.vec_n, p.rows > 1, h[u]);
         }
-    }
-    y = channel_sum<L>(y);
-    if (in && n0 == 0) {
-        if (on) {
-            if (p.D) y = fmaf(p.D[c], x, y);
-            if (p.z) {
-                const float z = to_float(((const T*)p.z)[b * p.zb + c]);
-                y *= z * sigmoid(z);
+        y = channel_sum<L>(y);
+        if (in[u] && n0 == 0) {
+            if (on[u]) {
+                y = fmaf(D, to_float(x[u]), y);
+                if (p.z) y *= to_float(z[u]) * sigmoid(to_float(z[u]));
             }
+            ((T*)p.y)[row] = from_float<T>(on[u] ? y : 0.f);
         }
-        ((T*)p.y)[row] = from_float<T>(on ? y : 0.f);
     }
 }
 
@@ -1624,7 +1663,8 @@ Tensor selective_step(Tensor state, const Tensor& x_in, const Tensor& dt_in, con
     p.vec_n = p.states % 4 == 0 && aligned(state, 4) && aligned(A, 4);
     p.vec_b = p.states % 4 == 0 && aligned(B, 4) && aligned(C, 4);
     const int l = lanes_for(p.states);
-    const int64_t n = blocks_for(p.batch * p.width * l, op);
+    p.rows = p.batch * p.width * l < 1 << 20 ? 1 : SR;
+    const int64_t n = blocks_for((p.batch + p.rows - 1) / p.rows * p.width * l, op);
     by_scan(x, l, [&](auto t, auto k) {
         hipLaunchKernelGGL((scan_step_kernel<decltype(t), decltype(k)::value>), dim3(n),
                            dim3(256), 0, at::cuda::getCurrentCUDAStream(), p);
