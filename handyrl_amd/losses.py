@@ -119,9 +119,10 @@ def clipped_policy_loss(logits, actions, old_log_probs, advantages, mask=None,
     the CPU).
 
     Returns (loss, stats): a float32 scalar and the detached sums
-    ``POLICY_LOSS_STATS``: surrogate loss, KL, entropy, scaled entropy,
-    clipped rows and the mask's sum, each weighted by the mask.  The gradient
-    cannot be differentiated again.
+    ``POLICY_LOSS_STATS``: surrogate loss, KL, entropy and scaled entropy
+    (weighted by the mask), the number of clipped rows, and the mask's sum.
+    The gradient cannot be differentiated again, and a backward pass can only be
+    captured into a graph if its forward pass was.
     """
     clip_high = clip if clip_high is None else clip_high
     if not 0 <= clip <= 1 or not clip_high >= 0:
@@ -165,17 +166,22 @@ def clipped_policy_loss(logits, actions, old_log_probs, advantages, mask=None,
     logp = F.log_softmax(torch.where(on.unsqueeze(-1), logits.to(real), 0), dim=-1)
     taken = torch.where(on, actions, 0).unsqueeze(-1)
     x = torch.where(on, logp.gather(-1, taken).squeeze(-1) - old, 0)
-    ratio = x.exp()
     adv = torch.where(on, adv, 0)
-    surrogate = torch.min(ratio * adv, ratio.clamp(1 - clip, 1 + clip_high) * adv)
+    now = x.detach().exp()
+    flat = ((adv > 0) & (now > 1 + clip_high)) | ((adv < 0) & (now < 1 - clip))
+    # the minimum, written so that a ratio without a part in it cannot spoil
+    # the gradient by overflowing
+    surrogate = adv * torch.where(flat, now.clamp(1 - clip, 1 + clip_high),
+                                  torch.where(flat, 0, x).exp())
     kl = torch.expm1(x) - x
     p = logp.exp()
     entropy = -torch.where(p > 0, p * logp.clamp(min=torch.finfo(real).min), 0).sum(-1)
     scale = torch.where(on, scale, 0)
     terms = [-surrogate * mask, kl * mask, entropy * mask, entropy * mask * scale]
     p_sum, kl_sum, ent_sum, scaled_sum = [t.sum() for t in terms]
-    loss = p_sum + kl_coef * kl_sum - entropy_coef * scaled_sum
-    flat = ((adv > 0) & (ratio > 1 + clip_high)) | ((adv < 0) & (ratio < 1 - clip))
+    loss = p_sum - entropy_coef * scaled_sum
+    if kl_coef != 0:                # a ratio that overflows only counts where it is asked for
+        loss = loss + kl_coef * kl_sum
     stats = torch.stack([p_sum, kl_sum, ent_sum, scaled_sum,
-                         (on & flat).sum().to(real), mask.sum()]).detach()
+                         flat.sum().to(real), mask.sum()]).detach()
     return loss, stats

@@ -117,7 +117,8 @@ __device__ __forceinline__ Row row_terms(const LossArgs& p, float m, float escal
     r.surrogate = flat ? bound * adv : ratio * adv;
     r.kl = exp_rest(x, ratio);
     r.clipped = flat ? 1.f : 0.f;
-    r.pull = m * ((flat ? 0.f : -ratio * adv) + p.beta * (ratio - 1.f));
+    r.pull = m * ((flat ? 0.f : -ratio * adv) +
+                  (p.beta != 0.f ? p.beta * (ratio - 1.f) : 0.f));      // not 0 * inf
     // with p_j = e / S0 and log p_j = x - log S0:
     //   -pull p_j + w p_j (log p_j + H) = e / S0 (w x + w (H - log S0) - pull)
     const float w = m * p.gamma * escale;
@@ -379,7 +380,8 @@ __global__ __launch_bounds__(256) void policy_loss_finish_kernel(
     }
     if (threadIdx.x < kStats) stats[threadIdx.x] = (float)s[0][threadIdx.x];
     if (threadIdx.x == 0)
-        loss[0] = (float)(s[0][0] + (double)beta * s[0][1] - (double)gamma * s[0][3]);
+        loss[0] = (float)(s[0][0] + (beta != 0.f ? (double)beta * s[0][1] : 0.) -
+                          (double)gamma * s[0][3]);
 }
 
 // One value a row: `t` has the rows' shape, perhaps with a last axis of 1, or
@@ -567,8 +569,11 @@ public:
             grad = ctx->saved_data["grad"].toTensor();
             ctx->saved_data["grad"] = c10::IValue();
         }
-        const bool ready = grad.defined() &&
-            ctx->saved_data["capture"].toInt() == (int64_t)capture_of(stream);
+        const int64_t then = ctx->saved_data["capture"].toInt(), now = capture_of(stream);
+        // the leaves' own streams would be drawn into the capture and never joined
+        TORCH_CHECK(then != 0 || now == 0, "clipped_policy_loss: a captured backward pass needs "
+                    "a captured forward pass");
+        const bool ready = grad.defined() && then == now;
         if (!ready) grad = torch::empty(logits.sizes(), logits.options());
         const auto flat = as_rows(logits);
         const auto up = grads[0].to(torch::kFloat32);

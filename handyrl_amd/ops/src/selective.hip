@@ -106,6 +106,15 @@ struct ConvArgs {
     int width, tile, tiles, nparts, silu;
 };
 
+// Whether none of the 64 steps from `mask` on is observed.
+__device__ __forceinline__ bool none_of_64(const bool* mask) {
+    unsigned long long w[8], any = 0;
+    __builtin_memcpy(w, mask, 64);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= w[i];
+    return any == 0;
+}
+
 // The last K-1 observed inputs before t0, oldest first.
 template <typename T, int K, int V>
 __device__ __forceinline__ void conv_behind(const ConvArgs& p, long b, long t0, int c,
@@ -121,9 +130,13 @@ __device__ __forceinline__ void conv_behind(const ConvArgs& p, long b, long t0, 
         }
         if (near) return;
     }
-    int need = K - 2;
+    int need = K - 2, unseen = 0;
     for (long t = t0 - 1; t >= 0 && need >= 0; --t) {
-        if (mask && !mask[t]) continue;
+        if (mask && !mask[t]) {         // through a long gap 64 steps at a time
+            if (++unseen >= 16 && t >= 64 && none_of_64(mask + t - 64)) t -= 64;
+            continue;
+        }
+        unseen = 0;
         float v[V];
         load_pack<T, V>(x + t * p.xt, v);
 #pragma unroll
@@ -289,8 +302,21 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
             else if (to <= carried && p.last)
                 store_pack<T, V>((T*)p.last + (b * (K - 1) + carried - to) * p.width + c, g);
         };
-        int ahead = 0;
+        int ahead = 0, unseen = 0;
         for (long t = t0; t < p.steps && ahead < K - 1; t += CU) {
+            if (t >= t1) {
+                bool pending = false;   // does an input of the tile wait for more steps?
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) pending = pending || place[k] != none;
+                if (!pending) break;
+                if (unseen >= 16 && mask) {             // a long gap: 64 steps at a time
+                    const long from = t;
+                    while (t + 64 <= p.steps && none_of_64(mask + t)) t += 64;
+                    if (t >= p.steps) break;
+                    if (t > from) fetch(t);
+                    unseen = 0;
+                }
+            }
             Pack<T, V> cx[CU], cg[CU];
             bool on[CU];
 #pragma unroll
@@ -307,8 +333,10 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
                 if (!on[u]) {
                     const float zero[V] = {};
                     if (own) store_pack<T, V>(dx + (t + u - t0) * p.width, zero);
+                    ++unseen;
                     continue;
                 }
+                unseen = 0;
                 if (!own) ++ahead;
                 float first[V];
 #pragma unroll
@@ -1171,6 +1199,23 @@ template <typename F> void by_type(const Tensor& x, F f)
 }
 template <int N> struct Const { static constexpr int value = N; };
 
+// The capture that the current stream is in, or 0.
+int64_t capture_now()
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_HIP_CHECK(hipStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(), &status, &id));
+    return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
+// A captured backward pass of an eager forward pass would draw the leaves' own
+// streams into the capture, which never join it.
+void check_capture(const char* op, const torch::autograd::AutogradContext* ctx)
+{
+    TORCH_CHECK(ctx->saved_data.at("capture").toInt() != 0 || capture_now() == 0, op,
+                ": a captured backward pass needs a captured forward pass");
+}
+
 // A step changes the state behind torch's back: tell autograd's version check.
 void moved_on(const Tensor& state) {
     if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
@@ -1263,7 +1308,9 @@ public:
         const auto bias = bias_in.value_or(Tensor()), state = state_in.value_or(Tensor()),
                    mask = mask_in.value_or(Tensor());
         ctx->save_for_backward({x, w, bias, state, mask});
+        const c10::DeviceGuard guard(x.device());
         ctx->saved_data["silu"] = silu;
+        ctx->saved_data["capture"] = capture_now();
         ctx->set_materialize_grads(false);
         return conv_forward(x, w, bias, state, mask, silu);
     }
@@ -1276,6 +1323,7 @@ public:
         auto saved = ctx->get_saved_variables();
         const auto &x = saved[0], &w = saved[1], &bias = saved[2], &state = saved[3];
         const c10::DeviceGuard guard(x.device());
+        check_capture("causal_conv", ctx);
         auto stream = at::cuda::getCurrentCUDAStream();
         const int64_t taps = w.size(1);
         auto dy = grads[0].defined() ? grads[0].contiguous()
@@ -1513,7 +1561,9 @@ public:
         auto out = scan_forward(s, true);
         ctx->save_for_backward({s.x, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.state, s.mask,
                                 out[2]});
+        const c10::DeviceGuard guard(x.device());
         ctx->saved_data["softplus"] = softplus;
+        ctx->saved_data["capture"] = capture_now();
         ctx->set_materialize_grads(false);
         return {out[0], out[1]};
     }
@@ -1528,6 +1578,7 @@ public:
                  ctx->saved_data["softplus"].toBool()};
         const auto& ckpt = v[10];
         const c10::DeviceGuard guard(s.x.device());
+        check_capture("selective_scan", ctx);
         auto stream = at::cuda::getCurrentCUDAStream();
         ScanArgs p = scan_args(s);
         auto fp32 = s.A.options();

@@ -111,7 +111,7 @@ def _window_prediction(model, hidden, observations, batch, args):
     window = getattr(model, 'model', model).forward_window
     rows = map_r(observations, lambda o: o.expand(-1, -1, P, *[-1] * (o.dim() - 3))
                  .transpose(1, 2).flatten(0, 1))
-    mask = omask.view(B, T, P).transpose(1, 2).flatten(0, 1) != 0
+    mask = omask.reshape(B, T, P).transpose(1, 2).flatten(0, 1) != 0
     hidden = map_r(hidden, lambda h: h.flatten(0, 1))
     cut, parts = args['burn_in_steps'], []
     if cut > 0:

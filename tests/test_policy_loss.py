@@ -115,6 +115,22 @@ def test_broadcasts_and_trailing_axis():
     assert loss.item() == want.item()
 
 
+def check_overflow(device):
+    """Without a KL term a ratio that overflows counts as the clipped one where
+    the surrogate is flat."""
+    args = make((8,), 5, device=device)
+    args['mask'][:] = 1
+    args['advantages'][2], args['old_log_probs'][2] = 1.5, -500.0
+    z = args['logits'].requires_grad_()
+    loss, stats = clipped_policy_loss(**args, clip=0.2, kl_coef=0.0, entropy_coef=0.1)
+    loss.backward()
+    assert loss.isfinite() and z.grad.isfinite().all() and math.isinf(stats[1].item())
+
+
+def test_eager_overflow():
+    check_overflow('cpu')
+
+
 REFUSALS = [
     (dict(clip=-0.1), 'clip must be'), (dict(clip=1.5), 'clip must be'),
     (dict(clip_high=-1.0), 'clip_high'),
@@ -298,6 +314,30 @@ def test_kernel_in_a_graph(rows, width):
         graph.replay()
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+@gpu
+def test_kernel_overflow():
+    check_overflow('cuda')
+
+
+@gpu
+def test_kernel_forward_and_backward_in_graphs_of_their_own():
+    """As make_graphed_callables has them, with one upstream gradient and another."""
+    args = make((64,), 214, device='cuda')
+    logits = args.pop('logits')
+
+    class Loss(torch.nn.Module):
+        def forward(self, z):
+            return clipped_policy_loss(z, **args, **COEFS)[0]
+
+    z = logits.clone().requires_grad_()
+    want, = torch.autograd.grad(Loss()(z), z)
+    graphed = torch.cuda.make_graphed_callables(Loss(), (torch.zeros_like(logits).requires_grad_(),))
+    for scale in (1.0, 2.0, 1.0, -0.5):          # powers of two: products without rounding
+        z = logits.clone().requires_grad_()
+        got, = torch.autograd.grad(graphed(z) * scale, z)
+        assert torch.equal(got, want * scale)
 
 
 @gpu

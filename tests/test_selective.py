@@ -465,6 +465,19 @@ def test_conv_matches_64_bits(case, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('where', [[], [0], [3, 4, 5, 6], [0, 1, 399], [2, 150, 151, 290], [399]])
+def test_conv_through_long_gaps(where):
+    a, grads = make_conv(2, 400, 6, 4)
+    a['mask'][0] = False
+    a['mask'][0, where] = True
+    assert_conv(a, *grads)
+    a, grads = make_scan(2, 400, 6, 4)
+    a['mask'][0] = False
+    a['mask'][0, where] = True
+    assert_scan(a, *grads)
+
+
+@gpu
 def test_kernel_holes():
     check_holes('cuda')
 
