@@ -156,6 +156,8 @@ __device__ __forceinline__ void add_row(double* sum, const Row& r, const RowIn& 
 }
 
 // Rows of up to 64 E values: G lanes a row, the row in registers, E a lane.
+// 16384x214 fp32: 12 us with the gradient (28 MB; launch and latency are 3 of
+// them), 13 + 13 with a kernel each way that reads the row three times.
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void policy_rows_kernel(LossArgs p)
 {
@@ -260,7 +262,9 @@ template <typename T> struct Vec {
 // taken 16 bytes a lane at a time: CH such pieces a lane stay in registers, so
 // that the row is read once; CH = 0 walks rows of any width and reads them
 // again.  The few values before the first border and behind the last are one
-// more value each for the first lanes.
+// more value each for the first lanes.  Memory bounds it: 4096x32003 bf16 takes
+// 123 us with the gradient, 4.3 TB/s where a copy reaches 5.1 (1036 us in two
+// kernels that read the row seven times).
 template <typename T, int NT, int CH>
 __global__ __launch_bounds__(NT, 1024 / NT) void policy_wide_kernel(LossArgs p)
 {

@@ -186,7 +186,9 @@ __device__ __forceinline__ void conv_weights(const ConvArgs& p, int c, float (&w
 
 constexpr int CU = 4;           // steps that a lane fetches at once
 
-// A lane walks V channels of one tile of steps with the window in registers.
+// A lane walks V channels of one tile of steps with the window in registers, so
+// each input is read once but for the K-1 before each tile.  Memory bounds it:
+// 4x4099x2048 bf16 takes 27 us on the GPU, 4.9 TB/s where a copy reaches 5.1.
 template <typename T, int K, int V>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
 {
@@ -257,7 +259,8 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
 // Backward: the lane walks its tile and K-1 observed steps behind it, so that
 // every input of the tile has met all steps that used it.  Each input of the
 // window has its gradient so far and its place: a step of the tile, none
-// (another tile's), or one of the carried inputs.
+// (another tile's), or one of the carried inputs.  128x16x512 takes 13 us, the
+// time of 16 steps one behind the other, and the sum over its parts 4.
 template <typename T, int K, int V>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
 {
@@ -684,7 +687,10 @@ struct StepIn {
 
 // LOCAL: the segment's own end from a zero start, and its sum of d, for the
 // segments behind it.  Otherwise the outputs, from the state before the
-// segment: the carried one moved through the segments before.
+// segment: the carried one moved through the segments before.  Vector
+// instructions bound both: 17 and 23 a step of four states, and 0.3 as many to
+// stage a chunk.  4x2048x2048 with 16 states, 8 segments: 64 and 110 us (of the
+// memory's rate they take 0.5 and 2.6 TB/s).
 template <typename T, int L, bool LOCAL>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
 {
@@ -780,7 +786,9 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
 //   lam_t = C_t g_t + carry,  carry <- exp(d_t A) lam_t
 // LOCAL: a segment's carry from a zero one behind it.  Otherwise the
 // gradients: h is walked again from a kept state and stays in registers with
-// exp(d A), then the same steps are walked backwards.
+// exp(d A), then the same steps are walked backwards.  4x2048x2048 with 16
+// states, 8 segments: 74 and 322 us; of the latter's issue slots vector
+// instructions take 65 to 70 %, a fifth of them to stage and to store a chunk.
 // Eight steps of states and decays at a time stay below 256 registers: 593 us
 // for training 4x2048x2048 against 633 with sixteen, which spill.
 template <typename T, int L, bool LOCAL>
