@@ -155,3 +155,81 @@ def test_training_step():
 @pytest.mark.parametrize('bf16', [False, True])
 def test_training_step_gpu(bf16):
     check_training('cuda', bf16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bf16', [False, True])
+def test_captured_window_training_gpu(bf16):
+    """The core, the heads and the clipped loss with all gradients in one graph,
+    replayed on batches of other episodes, against the eager passes."""
+    torch.manual_seed(5)
+    args = make_args(burn_in_steps=2)
+    net = WindowNet()
+    batches = []
+    for k in range(3):
+        random.seed(k)
+        batch = played(net, {**args, 'seed': k}, n=3 + k)
+        batches.append(map_r(batch, lambda v: v.cuda()))
+    net = net.cuda()
+    model = ModelWrapper(net)
+    static = map_r(batches[0], lambda v: v.clone())
+    hidden = model.init_hidden([static['value'].size(0), static['value'].size(2)])
+
+    def run():
+        with torch.autocast('cuda', dtype=torch.bfloat16, enabled=bf16, cache_enabled=False):
+            losses, dcnt = compute_loss(static, model, hidden, args)
+        grads = torch.autograd.grad(losses['total'], list(net.parameters()))
+        return [v.detach() for v in (*losses.values(), dcnt, *grads)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for batch in (batches[1], batches[2], batches[0]):
+        for k in static:
+            static[k].copy_(batch[k])
+        eager = [v.clone() for v in run()]
+        torch.cuda.synchronize()
+        graph.replay()
+        assert len(out) == len(eager) and all(v.isfinite().all() for v in eager)
+        for a, b in zip(out, eager):
+            # library products may be taken in another order by the graph: sums of some
+            # 50 terms of order 1 in the losses, of as many rows in the gradients
+            torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-4 + 1e-3 * float(b.abs().max()))
+
+
+@pytest.mark.gpu
+def test_clipped_loss_in_the_captured_learner_gpu():
+    """The learner's captured step on the device replay with policy_loss 'CLIP'."""
+    from handyrl_amd.actor import GeeseActorPool
+    from handyrl_amd.hipgraph import GraphedReplayTrainStep
+    from handyrl_amd.models.geese_net import GeeseNet
+    from handyrl_amd.replay import DeviceReplay
+    args = make_args(turn_based_training=False, forward_steps=8, batch_size=16, bf16=True,
+                     policy_target='VTRACE', value_target='VTRACE', compress_episodes=False,
+                     maximum_episodes=500)
+    device = torch.device('cuda', 0)
+    trainer = Trainer(args, GeeseNet(), device=device, batcher=False)
+    pool = GeeseActorPool(trainer.model, args, n_games=64, device=device, seed=0)
+    trainer.model.eval()
+    for _ in range(40000):
+        pool.step_once()
+        if pool.episodes_done >= 40:
+            break
+    assert pool.episodes_done >= 40, 'no episodes finished'
+    replay = DeviceReplay(args, device, bytes_budget=256 << 20)
+    replay.extend(pool.harvest())
+    step = GraphedReplayTrainStep(trainer, replay, args['batch_size'])
+    assert step.graph is not None, 'capture must succeed at world_size 1'
+    before = [p.detach().clone() for p in trainer.params]
+    for _ in range(3):
+        losses, dcnt = step.step()
+        torch.cuda.synchronize()
+        assert all(v.isfinite() for v in losses.values()) and float(dcnt) > 0
+    assert {'p', 'v', 'kl', 'clip', 'ent', 'total'} == set(losses)
+    assert any(not torch.equal(b, p.detach()) for b, p in zip(before, trainer.params))

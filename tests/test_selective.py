@@ -471,6 +471,10 @@ def test_conv_through_long_gaps(where):
     a['mask'][0] = False
     a['mask'][0, where] = True
     assert_conv(a, *grads)
+    a, grads = make_conv(3, 413, 3, 3)          # rows of the mask begin at odd addresses
+    a['mask'][1] = False
+    a['mask'][1, where] = True
+    assert_conv(a, *grads)
     a, grads = make_scan(2, 400, 6, 4)
     a['mask'][0] = False
     a['mask'][0, where] = True
