@@ -178,21 +178,32 @@ def assert_matches_64_bits(args, grad_out=1.0):
     (want * grad_out).backward()
 
     width = z.size(-1)
-    finite = ref['logits'].detach().clamp(min=-60)
-    reach = float(finite.max() - finite.min()) + float(ref['old_log_probs'].abs().max()) \
-        if finite.numel() else 0
-    rel = STEP * (8 + 2 * reach + width / 64)       # of one row's ratio or probability
+    rel = relative_error(ref)
     adv = ref['advantages'].abs() + 1
     m = ref['mask'].abs()
     size = float((m * (2 * adv + 3 + math.log(width + 1))).sum()) if m.numel() else 0
     assert abs(loss.item() - want.item()) <= 4 * rel * size + STEP * abs(want.item())
     assert torch.all((stats.cpu().double() - sums).abs() <= 4 * rel * size + STEP * sums.abs())
-    per = (m * (3 * adv + math.log(width + 1))).unsqueeze(-1) * abs(grad_out)
-    off = (z.grad.cpu().double() - z64.grad).abs()
-    out = torch.finfo(z.dtype).eps / 2
     assert z.grad.dtype == z.dtype and z.grad.shape == z.shape
-    assert torch.all(off <= 4 * rel * per + out * z64.grad.abs()), float((off / per).nan_to_num().max())
+    assert_gradient(z.grad, z64.grad, ref, grad_out)
     return loss, z.grad
+
+
+def relative_error(ref):
+    """Of one row's ratio or probability."""
+    finite = ref['logits'].detach().clamp(min=-60)
+    reach = float(finite.max() - finite.min()) + float(ref['old_log_probs'].abs().max()) \
+        if finite.numel() else 0
+    return STEP * (8 + 2 * reach + finite.size(-1) / 64)
+
+
+def assert_gradient(grad, want, ref, grad_out=1.0):
+    adv, m = ref['advantages'].abs() + 1, ref['mask'].abs()
+    per = (m * (3 * adv + math.log(grad.size(-1) + 1))).unsqueeze(-1) * abs(grad_out)
+    off = (grad.cpu().double() - want).abs()
+    out = torch.finfo(grad.dtype).eps / 2
+    assert torch.all(off <= 4 * relative_error(ref) * per + out * want.abs()), \
+        float((off / per).nan_to_num().max())
 
 
 @gpu
@@ -345,3 +356,26 @@ def test_kernel_results_repeat():
     args = make((5000,), 37, device='cuda')
     runs = [clipped_policy_loss(**args, **COEFS) for _ in range(3)]
     assert all(torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1]) for r in runs)
+
+
+@gpu
+def test_kernel_past_32_bit_offsets():
+    """2.2e9 logits: the last rows as they come alone."""
+    rows, width = 70000, 32003
+    z = torch.empty(rows, width, device='cuda', dtype=torch.bfloat16).normal_().requires_grad_()
+    args = dict(actions=torch.randint(0, width, (rows,), device='cuda'),
+                old_log_probs=torch.full((rows,), -10.5, device='cuda'),
+                advantages=torch.randn(rows, device='cuda'),
+                mask=(torch.arange(rows, device='cuda') % 3 > 0).float())
+    loss, stats = clipped_policy_loss(z, **args, **COEFS)
+    grad, = torch.autograd.grad(loss, z)
+    # alone, a row may begin elsewhere between 16 byte borders and be summed in another
+    # order, so the last rows are held to the formula in 64 bits
+    tail = slice(rows - 40, rows)
+    ref = in64({'logits': z[tail], **{k: v[tail] for k, v in args.items()}})
+    z64 = ref['logits'].requires_grad_()
+    want, _ = clipped_policy_loss(**ref, **COEFS)
+    want.backward()
+    assert_gradient(grad[tail], z64.grad, ref)
+    assert stats[5].item() == args['mask'].sum().item()
+    assert (grad[::3][:5] == 0).all() and grad[1].abs().sum() > 0

@@ -618,3 +618,32 @@ def test_kernels_in_a_graph_and_on_a_side_stream():
         graph.replay()
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+@gpu
+def test_kernels_past_32_bit_offsets():
+    """2.4e9 values a tensor: the last row as it comes alone."""
+    shape = (3, 1 << 20, 768)
+    g = torch.Generator('cuda').manual_seed(0)
+    wide = torch.randn(shape[1:], device='cuda', generator=g).bfloat16()
+    x = torch.empty(shape, device='cuda', dtype=torch.bfloat16)
+    for b in range(3):
+        x[b] = wide.roll(b, 0)
+    weight = torch.randn(768, 4, device='cuda', generator=g)
+    y, last = causal_conv(x, weight, activation='silu')
+    one, end = causal_conv(x[2:], weight, activation='silu')
+    assert torch.equal(y[2], one[0]) and torch.equal(last[2], end[0])
+    del one
+    A = -torch.rand(768, 2, device='cuda', generator=g) - 0.5
+    B = torch.randn(3, shape[1], 2, device='cuda', generator=g).bfloat16()
+    leaf = x.requires_grad_()
+    out, state = selective_scan(leaf, y, A, B, B, dt_softplus=True)
+    dx, = torch.autograd.grad(out, leaf, y)
+    alone = x.detach()[2:].requires_grad_()
+    one, end = selective_scan(alone, y[2:], A, B[2:], B[2:], dt_softplus=True)
+    d_one, = torch.autograd.grad(one, alone, y[2:])
+    # another cut into segments: a rounding to bfloat16 may fall the other way
+    for a, b in ((out[2], one[0]), (dx[2], d_one[0])):
+        for part in (slice(0, 4096), slice(-4096, None)):
+            torch.testing.assert_close(a[part], b[part], rtol=2 ** -6, atol=1e-3)
+    torch.testing.assert_close(state[2], end[0], rtol=1e-4, atol=1e-4)
