@@ -109,52 +109,61 @@ struct ConvArgs {
     int width, tile, tiles, nparts, silu;
 };
 
-// Whether none of the 64 steps from `mask` on is observed.
-__device__ __forceinline__ bool none_of_64(const bool* mask) {
-    unsigned long long w[8], any = 0;
-    __builtin_memcpy(w, mask, 64);
+// The masks of the 64 steps from `from` on as bits; 0 for steps outside [0, steps).
+// The product gathers the low bits of eight bytes into one without a carry.
+__device__ __forceinline__ unsigned long long seen_64(const bool* mask, long from, long steps) {
+    unsigned long long bits = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) any |= w[i];
-    return any == 0;
+    for (int g = 0; g < 8; ++g) {
+        const long t = from + 8 * g;
+        unsigned long long w = 0;
+        if (t >= 0 && t + 8 <= steps) {
+            __builtin_memcpy(&w, mask + t, 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (t + i >= 0 && t + i < steps) w |= (unsigned long long)mask[t + i] << (8 * i);
+        }
+        bits |= ((w * 0x0102040810204080ull) >> 56) << (8 * g);
+    }
+    return bits;
 }
 
 // The last K-1 observed inputs before t0, oldest first.
-template <typename T, int K, int V>
+template <typename T, int K, int V, bool MASKED>
 __device__ __forceinline__ void conv_behind(const ConvArgs& p, long b, long t0, int c,
                                             float (&win)[K - 1][V]) {
     const T* x = (const T*)p.x + b * p.xb + c;
-    const bool* mask = p.mask ? p.mask + b * p.steps : nullptr;
-    bool near = t0 >= K - 1;            // the K-1 steps before, where all of them are observed
-    if (near) {
+    long at[K - 1];
+    int need = K - 1;                   // the oldest `need` are not found yet
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) {
-            load_pack<T, V>(x + (t0 - (K - 1) + k) * p.xt, win[k]);
-            if (mask) near = near && mask[t0 - (K - 1) + k];
+    for (int k = 0; k < K - 1; ++k) at[k] = -1;
+    if (!MASKED) {
+        need = t0 < K - 1 ? (int)(K - 1 - t0) : 0;
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) at[k] = t0 - (K - 1) + k;
+    } else {
+        const bool* mask = p.mask + b * p.steps;
+        for (long end = t0; end > 0 && need > 0; end -= 64) {
+            unsigned long long bits = seen_64(mask, end - 64, p.steps);
+            if (bits && end < 64) bits &= ~0ull << (64 - end);
+#pragma unroll
+            for (int k = K - 2; k >= 0; --k) {
+                if (k != need - 1 || !bits) continue;
+                const int top = 63 - __clzll(bits);
+                at[k] = end - 64 + top;
+                bits ^= 1ull << top;
+                --need;
+            }
         }
-        if (near) return;
     }
-    int need = K - 2, unseen = 0;
-    for (long t = t0 - 1; t >= 0 && need >= 0; --t) {
-        if (mask && !mask[t]) {         // through a long gap 64 steps at a time
-            if (++unseen >= 16 && t >= 64 && none_of_64(mask + t - 64)) t -= 64;
-            continue;
-        }
-        unseen = 0;
-        float v[V];
-        load_pack<T, V>(x + t * p.xt, v);
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k)
-            if (k == need)
-#pragma unroll
-                for (int i = 0; i < V; ++i) win[k][i] = v[i];
-        --need;
-    }
-    const int found = K - 2 - need;
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-        if (k > need) continue;
-        if (p.state) {
-            load_pack<T, V>((const T*)p.state + (b * (K - 1) + k + found) * p.width + c, win[k]);
+        if (k >= need) {
+            load_pack<T, V>(x + at[k] * p.xt, win[k]);
+        } else if (p.state) {
+            load_pack<T, V>((const T*)p.state + (b * (K - 1) + k + K - 1 - need) * p.width + c,
+                            win[k]);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) win[k][i] = 0.f;
@@ -188,8 +197,8 @@ constexpr int CU = 4;           // steps that a lane fetches at once
 
 // A lane walks V channels of one tile of steps with the window in registers, so
 // each input is read once but for the K-1 before each tile.  Memory bounds it:
-// 4x4099x2048 bf16 takes 27 us on the GPU, 4.9 TB/s where a copy reaches 5.1.
-template <typename T, int K, int V>
+// 4x4099x2048 bf16 takes 27.6 us on the GPU, 4.9 TB/s where a copy reaches 5.1.
+template <typename T, int K, int V, bool MASKED>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
 {
     const unsigned lanes = p.width / V;
@@ -204,7 +213,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
     float w[K][V], bias[V], win[K - 1][V];
     const T* x = (const T*)p.x + b * p.xb + c;
     T* y = (T*)p.y + b * p.steps * p.width + c;
-    const bool* mask = p.mask ? p.mask + b * p.steps : nullptr;
+    const bool* mask = p.mask + b * p.steps;
     Pack<T, V> next[CU];
     bool next_on[CU];
     auto fetch = [&](long t) {
@@ -213,12 +222,12 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
             next_on[u] = t + u < t1;
             if (!next_on[u]) continue;
             next[u] = *(const Pack<T, V>*)(x + (t + u) * p.xt);
-            if (mask) next_on[u] = mask[t + u];
+            if (MASKED) next_on[u] = mask[t + u];
         }
     };
     fetch(t0);
     conv_weights<K, V>(p, c, w, bias);
-    conv_behind<T, K, V>(p, b, t0, c, win);
+    conv_behind<T, K, V, MASKED>(p, b, t0, c, win);
     for (long t = t0; t < t1; t += CU) {
         Pack<T, V> now[CU];
         bool on[CU];
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
 // window has its gradient so far and its place: a step of the tile, none
 // (another tile's), or one of the carried inputs.  128x16x512 takes 13 us, the
 // time of 16 steps one behind the other, and the sum over its parts 4.
-template <typename T, int K, int V>
+template <typename T, int K, int V, bool MASKED>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
 {
     const unsigned lanes = p.width / V;
@@ -281,7 +290,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
         const T* x = (const T*)p.x + b * p.xb + c;
         const T* dy = (const T*)p.dy + b * p.steps * p.width + c;
         T* dx = (T*)p.y + (b * p.steps + t0) * p.width + c;
-        const bool* mask = p.mask ? p.mask + b * p.steps : nullptr;
+        const bool* mask = p.mask + b * p.steps;
 
         float win[K - 1][V], acc[K - 1][V] = {};
         int place[K - 1];                               // steps from t0 on
@@ -290,39 +299,65 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
         auto fetch = [&](long t) {
 #pragma unroll
             for (int u = 0; u < CU; ++u) {
-                non[u] = t + u < p.steps;
+                non[u] = t + u < t1;
                 if (!non[u]) continue;
                 nx[u] = *(const Pack<T, V>*)(x + (t + u) * p.xt);
                 ng[u] = *(const Pack<T, V>*)(dy + (t + u) * p.width);
-                if (mask) non[u] = mask[t + u];
+                if (MASKED) non[u] = mask[t + u];
             }
         };
         fetch(t0);
-        conv_behind<T, K, V>(p, b, t0, c, win);
+        conv_behind<T, K, V, MASKED>(p, b, t0, c, win);
+        bool pending = false;                           // an input waits for more steps
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) place[k] = t0 == 0 ? carried - k : none;
-
+        for (int k = 0; k < K - 1; ++k) {
+            place[k] = t0 == 0 ? carried - k : none;
+            pending = pending || t0 == 0;
+        }
         auto emit = [&](int to, const float (&g)[V]) {
             if (to >= 0)
                 store_pack<T, V>(dx + (long)to * p.width, g);
             else if (to <= carried && p.last)
                 store_pack<T, V>((T*)p.last + (b * (K - 1) + carried - to) * p.width + c, g);
         };
-        int ahead = 0, unseen = 0;
-        for (long t = t0; t < p.steps && ahead < K - 1; t += CU) {
-            if (t >= t1) {
-                bool pending = false;   // does an input of the tile wait for more steps?
+        // one observed step: its part in the taps and in the window's gradients
+        auto step = [&](const Pack<T, V>& px, const Pack<T, V>& pg, int at) {
+            float first[V];
 #pragma unroll
-                for (int k = 0; k < K - 1; ++k) pending = pending || place[k] != none;
-                if (!pending) break;
-                if (unseen >= 16 && mask) {             // a long gap: 64 steps at a time
-                    const long from = t;
-                    while (t + 64 <= p.steps && none_of_64(mask + t)) t += 64;
-                    if (t >= p.steps) break;
-                    if (t > from) fetch(t);
-                    unseen = 0;
+            for (int i = 0; i < V; ++i) {
+                const float v = to_float(px.v[i]);
+                float g = to_float(pg.v[i]);
+                if (p.silu) {
+                    float s = bias[i];
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][i], win[k][i], s);
+                    s = fmaf(w[K - 1][i], v, s);
+                    const float sg = sigmoid(s);
+                    g *= sg * (1.f + s * (1.f - sg));
                 }
+                if (at != none) {
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) dw[k][i] = fmaf(g, win[k][i], dw[k][i]);
+                    dw[K - 1][i] = fmaf(g, v, dw[K - 1][i]);
+                    db[i] += g;
+                }
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) acc[k][i] = fmaf(w[k][i], g, acc[k][i]);
+                first[i] = acc[0][i];
+#pragma unroll
+                for (int k = 0; k < K - 2; ++k) {
+                    acc[k][i] = acc[k + 1][i];
+                    win[k][i] = win[k + 1][i];
+                }
+                acc[K - 2][i] = w[K - 1][i] * g;
+                win[K - 2][i] = v;
             }
+            emit(place[0], first);
+#pragma unroll
+            for (int k = 0; k < K - 2; ++k) place[k] = place[k + 1];
+            place[K - 2] = at;
+        };
+        for (long t = t0; t < t1; t += CU) {
             Pack<T, V> cx[CU], cg[CU];
             bool on[CU];
 #pragma unroll
@@ -331,54 +366,49 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
                 cg[u] = ng[u];
                 on[u] = non[u];
             }
-            if (t + CU < t1 || t1 < p.steps) fetch(t + CU);
+            fetch(t + CU);
 #pragma unroll
             for (int u = 0; u < CU; ++u) {
-                if (t + u >= p.steps || ahead >= K - 1) break;
-                const bool own = t + u < t1;
-                if (!on[u]) {
+                if (t + u >= t1) break;
+                if (on[u]) {
+                    step(cx[u], cg[u], (int)(t + u - t0));
+                    pending = true;
+                } else {
                     const float zero[V] = {};
-                    if (own) store_pack<T, V>(dx + (t + u - t0) * p.width, zero);
-                    ++unseen;
-                    continue;
+                    store_pack<T, V>(dx + (t + u - t0) * p.width, zero);
                 }
-                unseen = 0;
-                if (!own) ++ahead;
-                float first[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float v = to_float(cx[u].v[i]);
-                    float g = to_float(cg[u].v[i]);
-                    if (p.silu) {
-                        float s = bias[i];
-#pragma unroll
-                        for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][i], win[k][i], s);
-                        s = fmaf(w[K - 1][i], v, s);
-                        const float sg = sigmoid(s);
-                        g *= sg * (1.f + s * (1.f - sg));
-                    }
-                    if (own) {
-#pragma unroll
-                        for (int k = 0; k < K - 1; ++k) dw[k][i] = fmaf(g, win[k][i], dw[k][i]);
-                        dw[K - 1][i] = fmaf(g, v, dw[K - 1][i]);
-                        db[i] += g;
-                    }
-#pragma unroll
-                    for (int k = 0; k < K - 1; ++k) acc[k][i] = fmaf(w[k][i], g, acc[k][i]);
-                    first[i] = acc[0][i];
-#pragma unroll
-                    for (int k = 0; k < K - 2; ++k) {
-                        acc[k][i] = acc[k + 1][i];
-                        win[k][i] = win[k + 1][i];
-                    }
-                    acc[K - 2][i] = w[K - 1][i] * g;
-                    win[K - 2][i] = v;
-                }
-                emit(place[0], first);
-#pragma unroll
-                for (int k = 0; k < K - 2; ++k) place[k] = place[k + 1];
-                place[K - 2] = own ? (int)(t + u - t0) : none;
             }
+        }
+        // the K-1 observed steps behind the tile, where an input of it waits for them
+        if (pending && t1 < p.steps) {
+            long at[K - 1];
+            int found = 0;
+            if (!MASKED) {
+                found = p.steps - t1 < K - 1 ? (int)(p.steps - t1) : K - 1;
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) at[k] = t1 + k;
+            } else {
+                for (long from = t1; from < p.steps && found < K - 1; from += 64) {
+                    unsigned long long bits = seen_64(mask, from, p.steps);
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) {
+                        if (k != found || !bits) continue;
+                        at[k] = from + __builtin_ctzll(bits);
+                        bits &= bits - 1;
+                        ++found;
+                    }
+                }
+            }
+            Pack<T, V> ax[K - 1], ag[K - 1];
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) {
+                if (k >= found) continue;
+                ax[k] = *(const Pack<T, V>*)(x + at[k] * p.xt);
+                ag[k] = *(const Pack<T, V>*)(dy + at[k] * p.width);
+            }
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+                if (k < found) step(ax[k], ag[k], none);
         }
         // what the window still holds of this tile ended in the carried inputs
 #pragma unroll
@@ -1276,12 +1306,14 @@ int conv_channels(const Tensor& x, std::initializer_list<Tensor> others)
     return ok ? 2 : 1;
 }
 
-// Steps of a lane's tile: 64, or down to 16 where that leaves fewer than 2^19
-// lanes (4x4099x2048: 50 us with 2^16, 39 with 2^17, 32 with 2^19).
+// Steps of a lane's tile: 64, or down to 16 where that leaves fewer than 2^18
+// lanes (fp32 1x7178x902 with gaps: 32 us at 32 steps, 21 at 16; with lanes
+// enough, bf16 6x2735x975 with gaps: 48 us at 32, 59 at 16, where the walk for
+// the observed steps behind weighs more; 4x4099x2048: 28 us at either).
 void cut_conv(ConvArgs& p, int channels)
 {
     for (p.tile = 64; p.tile > 16; p.tile /= 2)
-        if (p.batch * (p.width / channels) * ((p.steps + p.tile - 1) / p.tile) >= 1 << 19) break;
+        if (p.batch * (p.width / channels) * ((p.steps + p.tile - 1) / p.tile) >= 1 << 18) break;
     p.tiles = (int)((p.steps + p.tile - 1) / p.tile);
 }
 
@@ -1303,8 +1335,12 @@ std::vector<Tensor> conv_forward(const Tensor& x, const Tensor& w, const Tensor&
     cut_conv(p, channels);
     by_conv(x, taps, channels, [&](auto t, auto k, auto v) {
         const int64_t n = blocks_for(p.batch * p.tiles * (p.width / v.value), "causal_conv");
-        hipLaunchKernelGGL((conv_fwd_kernel<decltype(t), decltype(k)::value, decltype(v)::value>),
-                           dim3(n), dim3(256), 0, stream, p);
+        if (p.mask)
+            hipLaunchKernelGGL((conv_fwd_kernel<decltype(t), decltype(k)::value,
+                                decltype(v)::value, true>), dim3(n), dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((conv_fwd_kernel<decltype(t), decltype(k)::value,
+                                decltype(v)::value, false>), dim3(n), dim3(256), 0, stream, p);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return {y, last};
@@ -1362,8 +1398,12 @@ public:
         p.parts = parts.data_ptr<float>();
         by_conv(x, taps, channels, [&](auto t, auto k, auto v) {
             const int64_t n = blocks_for((int64_t)p.nparts * (p.width / v.value), "causal_conv");
-            hipLaunchKernelGGL((conv_bwd_kernel<decltype(t), decltype(k)::value,
-                                decltype(v)::value>), dim3(n), dim3(256), 0, stream, p);
+            if (p.mask)
+                hipLaunchKernelGGL((conv_bwd_kernel<decltype(t), decltype(k)::value,
+                                    decltype(v)::value, true>), dim3(n), dim3(256), 0, stream, p);
+            else
+                hipLaunchKernelGGL((conv_bwd_kernel<decltype(t), decltype(k)::value,
+                                    decltype(v)::value, false>), dim3(n), dim3(256), 0, stream, p);
         });
         auto rest = db.defined() ? db : torch::empty({x.size(2)}, w.options());
         const int64_t cols = (taps + 1) * x.size(2);
