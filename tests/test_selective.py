@@ -647,3 +647,12 @@ def test_kernels_past_32_bit_offsets():
         for part in (slice(0, 4096), slice(-4096, None)):
             torch.testing.assert_close(a[part], b[part], rtol=2 ** -6, atol=1e-3)
     torch.testing.assert_close(state[2], end[0], rtol=1e-4, atol=1e-4)
+
+
+@gpu
+@pytest.mark.parametrize('share', [0.01, 0.05, 0.5, 0.98])
+@pytest.mark.parametrize('steps', [63, 64, 65, 127, 200])
+@pytest.mark.parametrize('taps', [2, 3, 4])
+def test_conv_through_sparse_masks(share, steps, taps):
+    a, grads = make_conv(5, steps, 5, taps, share=share, state=taps != 3, seed=steps)
+    assert_conv(a, *grads)
