@@ -1527,6 +1527,11 @@ void cut_steps(ScanArgs& p)
     const int64_t blocks = std::max<int64_t>(1, p.batch * p.groups * p.tiles);
     int64_t segs = std::max<int64_t>(1, std::min({target / blocks, p.chunks, (int64_t)64}));
     p.seg_chunks = (int)std::max<int64_t>(1, (p.chunks + segs - 1) / segs);
+    // Segments are walked twice, so they have to be shorter than half of the steps.
+    // On the GPU, training with and without: 100x80x256 111 and 76 us (two
+    // segments of 3 of 5 chunks), 37x67x200 82 and 76 (of 2 of 5), 4x64x200 34
+    // and 48 (of 1 of 4), 32x80x256 56 and 58 (of 1 of 5).
+    if (2 * p.seg_chunks + 1 >= p.chunks) p.seg_chunks = (int)std::max<int64_t>(1, p.chunks);
     p.segs = (unsigned)std::max<int64_t>(1, (p.chunks + p.seg_chunks - 1) / p.seg_chunks);
 }
 
