@@ -217,14 +217,14 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
     T* y = (T*)p.y + b * p.steps * p.width + c;
     const bool* mask = p.mask + b * p.steps;
     Pack<T, V> next[CU];
-    bool next_on[CU];
+    int next_on[CU];            // a byte: turned into a bool here, it would be waited for
     auto fetch = [&](long t) {
 #pragma unroll
         for (int u = 0; u < CU; ++u) {
             next_on[u] = t + u < t1;
             if (!next_on[u]) continue;
             next[u] = *(const Pack<T, V>*)(x + (t + u) * p.xt);
-            if (MASKED) next_on[u] = mask[t + u];
+            if (MASKED) next_on[u] = ((const unsigned char*)mask)[t + u];
         }
     };
     fetch(t0);
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
     conv_behind<T, K, V, MASKED>(p, b, t0, c, win);
     for (long t = t0; t < t1; t += CU) {
         Pack<T, V> now[CU];
-        bool on[CU];
+        int on[CU];
 #pragma unroll
         for (int u = 0; u < CU; ++u) {
             now[u] = next[u];
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
         for (int u = 0; u < CU; ++u) {
             if (t + u >= t1) break;
             float out[V] = {};
-            if (on[u]) {
+            if (on[u] & 1) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float v = to_float(now[u].v[i]);
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
         float win[K - 1][V], acc[K - 1][V] = {};
         int place[K - 1];                               // steps from t0 on
         Pack<T, V> nx[CU], ng[CU];
-        bool non[CU];
+        int non[CU];                                    // bytes, as a bool is waited for
         auto fetch = [&](long t) {
 #pragma unroll
             for (int u = 0; u < CU; ++u) {
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
                 if (!non[u]) continue;
                 nx[u] = *(const Pack<T, V>*)(x + (t + u) * p.xt);
                 ng[u] = *(const Pack<T, V>*)(dy + (t + u) * p.width);
-                if (MASKED) non[u] = mask[t + u];
+                if (MASKED) non[u] = ((const unsigned char*)mask)[t + u];
             }
         };
         fetch(t0);
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
         };
         for (long t = t0; t < t1; t += CU) {
             Pack<T, V> cx[CU], cg[CU];
-            bool on[CU];
+            int on[CU];
 #pragma unroll
             for (int u = 0; u < CU; ++u) {
                 cx[u] = nx[u];
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
 #pragma unroll
             for (int u = 0; u < CU; ++u) {
                 if (t + u >= t1) break;
-                if (on[u]) {
+                if (on[u] & 1) {
                     step(cx[u], cg[u], (int)(t + u - t0));
                     pending = true;
                 } else {
