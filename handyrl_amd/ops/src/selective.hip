@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p)
 // Backward: the lane walks its tile and K-1 observed steps behind it, so that
 // every input of the tile has met all steps that used it.  Each input of the
 // window has its gradient so far and its place: a step of the tile, none
-// (another tile's), or one of the carried inputs.  128x16x512 takes 13 us, the
+// (another tile's), or one of the carried inputs.  128x16x512 takes 12 us, the
 // time of 16 steps one behind the other, and the sum over its parts 4.
 template <typename T, int K, int V, bool MASKED>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
@@ -1309,9 +1309,9 @@ int conv_channels(const Tensor& x, std::initializer_list<Tensor> others)
 }
 
 // Steps of a lane's tile: 64, or down to 16 where that leaves fewer than 2^18
-// lanes (fp32 1x7178x902 with gaps: 32 us at 32 steps, 21 at 16; with lanes
-// enough, bf16 6x2735x975 with gaps: 48 us at 32, 59 at 16, where the walk for
-// the observed steps behind weighs more; 4x4099x2048: 28 us at either).
+// lanes.  With gaps, fp32 1x7178x902: 26 us at 64 steps, 21 at 32, 20 at 16; with
+// lanes enough, bf16 6x2735x975: 41 us at 64 and 32, 46 at 16, where the walk for
+// the observed steps behind weighs more.  4x4099x2048: 28 us at 64 as at 32.
 void cut_conv(ConvArgs& p, int channels)
 {
     for (p.tile = 64; p.tile > 16; p.tile /= 2)
