@@ -689,6 +689,16 @@ __device__ __forceinline__ void load_channels(const float* from, const Place<L>&
     for (int i = 0; i < 4; ++i) out[i] = from && q.c + i < at.nc ? from[at.c0 + q.c + i] : 0.f;
 }
 
+// h e^(ln2 p).  A whole segment's factor may pass the range of a float where its
+// product with a small state, or one of 0, does not, so p's whole part goes to the
+// exponent of the product; behind 600 the product of any float but 0 has left the
+// range.  A p that is not a number comes back in `e` below.
+__device__ __forceinline__ float grown(float h, float p) {
+    p = fminf(fmaxf(p, -600.f), 600.f);
+    const float whole = rintf(p);
+    return ldexpf(exp2_fast(p - whole) * h, (int)whole);
+}
+
 // Moves a state (or, backwards, the gradient of one) through whole segments.
 template <int L>
 __device__ __forceinline__ void join_segment(const ScanArgs& p, const Place<L>& at, int seg,
@@ -698,7 +708,7 @@ __device__ __forceinline__ void join_segment(const ScanArgs& p, const Place<L>& 
     load4(p.seg_h + at.state_at(p, row), at.nn, p.vec_n, e);
     const float d = p.seg_d[row * p.width + at.c0 + at.c];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_fast(A2[i] * d), h[i], e[i]);
+    for (int i = 0; i < 4; ++i) h[i] = grown(h[i], A2[i] * d) + e[i];
 }
 
 // What a lane reads of one step.  The next step's is read before the present one

@@ -1,0 +1,55 @@
+"""Selective scan and short convolution where they are easiest to get wrong:
+growth past a float's range, rates without bound, plans of several chunks a
+segment and of several rows a lane.  Helpers and tolerances are those of
+test_selective.py."""
+
+import pytest
+import torch
+
+from test_selective import STEP, make_scan, move, run_scan, scan_by_hand
+
+gpu = pytest.mark.gpu
+
+
+def assert_results(got, want, size, a):
+    """As assert_scan has it: k half steps of each result's sum of magnitudes."""
+    steps, width = a['x'].shape[1:]
+    for k, v in got.items():
+        out = torch.finfo(v.dtype).eps / 2
+        off = (v.double().cpu() - want[k]).abs()
+        tol = STEP * (4 * steps + 64 + width / 8) * size[k] + out * want[k].abs() + 1e-37
+        assert torch.all(off <= tol), (k, float((off / tol).max()))
+
+
+def growing(what, sign):
+    """States that grow by e^4 a step (or e^3.125), past a float's range within a
+    segment of 32 steps, where all results stay in it: zeros, with inputs in the
+    last 16 steps and gradients in the first 16; or a tiny state (or a tiny
+    gradient of the last one) that meets 32 observed steps.  Sign 1: rates above
+    0; sign -1: steps below it."""
+    zeros = what == 'zeros'
+    a, (dy, dlast) = make_scan(1, 1100, 24, 16, gate=False, state=not zeros, share=1.0, plain=True)
+    a['A'] = torch.full_like(a['A'], sign)
+    a['dt'] = torch.full_like(a['dt'], sign * (4.0 if zeros else 3.125))
+    if zeros:
+        a['x'][:, :-16] = 0
+        dy[:, 16:] = 0
+        return a, dy, torch.zeros_like(dlast)
+    a['mask'] = torch.zeros(1, 1100, dtype=torch.bool)
+    a['mask'][:, slice(0, 32) if what == 'tiny state' else slice(1056, 1088)] = True
+    a['x'] = torch.zeros_like(a['x'])
+    a['state'] *= 1e-36 if what == 'tiny state' else 1e-30
+    dlast *= 1e-30 if what == 'tiny state' else 1e-36
+    return a, torch.zeros_like(dy), dlast
+
+
+@gpu
+@pytest.mark.parametrize('sign', [1.0, -1.0])
+@pytest.mark.parametrize('what', ['zeros', 'tiny state', 'tiny gradient'])
+def test_scan_of_growing_states(what, sign):
+    a, dy, dlast = growing(what, sign)
+    want = run_scan(move(a, double=True), dy.double(), dlast.double())
+    assert all(v.float().isfinite().all() for v in want.values())
+    # the magnitudes are the same for either sign
+    size = scan_by_hand(growing(what, 1.0)[0], dy, dlast, absolute=True)
+    assert_results(run_scan(move(a, 'cuda'), dy.cuda(), dlast.cuda()), want, size, a)
