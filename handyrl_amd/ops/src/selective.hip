@@ -671,14 +671,21 @@ template <typename T, int L> struct Chunk {
     }
 };
 
-// A lane's rates, times log2(e).
+// A rate times log2(e).  One past a float's range, an infinite one among them, stays
+// at its end: a step of length 0, unobserved or behind the last, has to take 0 * rate.
+__device__ __forceinline__ float rate_of(float a) {
+    const float r = a * kLog2e, most = __FLT_MAX__;
+    return r > most ? most : r < -most ? -most : r;     // NaN stays
+}
+
+// A lane's rates.
 template <int L>
 __device__ __forceinline__ void load_rates(const ScanArgs& p, const Place<L>& at, float* A2) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) A2[i] = 0.f;
     if (at.nn > 0) load4(p.A + (long)(at.c0 + at.c) * p.states + at.n0, at.nn, p.vec_n, A2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A2[i] *= kLog2e;
+    for (int i = 0; i < 4; ++i) A2[i] = rate_of(A2[i]);
 }
 
 // A thread's four values of D or dt_bias; zeros where there are none.

@@ -6,6 +6,7 @@ test_selective.py."""
 import pytest
 import torch
 
+from handyrl_amd.models.selective import selective_scan, selective_step
 from test_selective import STEP, make_scan, move, run_scan, scan_by_hand
 
 gpu = pytest.mark.gpu
@@ -53,3 +54,25 @@ def test_scan_of_growing_states(what, sign):
     # the magnitudes are the same for either sign
     size = scan_by_hand(growing(what, 1.0)[0], dy, dlast, absolute=True)
     assert_results(run_scan(move(a, 'cuda'), dy.cuda(), dlast.cuda()), want, size, a)
+
+
+@gpu
+@pytest.mark.parametrize('rate', [-float('inf'), -3e38])
+@pytest.mark.parametrize('steps', [21, 700])
+def test_scan_forgets_at_once(rate, steps):
+    """States whose rate has no bound hold the last observed step alone, past
+    holes and behind an end within a chunk.  With rates of -1e30 instead, 64
+    bits give the same: decays of 0, times a rate that is finite."""
+    a, (dy, dlast) = make_scan(2, steps, 40, 8)
+    a['A'][::2, 1::3] = rate
+    finite = {**a, 'A': a['A'].clamp(min=-1e30)}
+    got = run_scan(move(a, 'cuda'), dy.cuda(), dlast.cuda())
+    want = run_scan(move(finite, double=True), dy.double(), dlast.double())
+    assert_results(got, want, scan_by_hand(finite, dy, dlast, absolute=True), a)
+    held, t = a['state'].cuda(), int(a['mask'][0].nonzero()[0])
+    row = {k: a[k][:, t].cuda() for k in ('x', 'dt', 'B', 'C', 'z', 'mask')}
+    rest = {k: a[k].cuda() if torch.is_tensor(a[k]) else a[k] for k in ('A', 'D', 'dt_bias', 'dt_softplus')}
+    _, last = selective_scan(**{k: v[:, None] for k, v in row.items()}, **rest, state=held)
+    selective_step(held, **row, **rest)
+    assert held.isfinite().all()
+    torch.testing.assert_close(held, last, rtol=64 * STEP, atol=64 * STEP * 10)
