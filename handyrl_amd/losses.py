@@ -121,8 +121,9 @@ def clipped_policy_loss(logits, actions, old_log_probs, advantages, mask=None,
     Returns (loss, stats): a float32 scalar and the detached sums
     ``POLICY_LOSS_STATS``: surrogate loss, KL, entropy and scaled entropy
     (weighted by the mask), the number of clipped rows, and the mask's sum.
-    The gradient cannot be differentiated again, and a backward pass can only be
-    captured into a graph if its forward pass was.
+    On the GPU the gradient cannot be differentiated again, there is no
+    forward-mode derivative, and a backward pass can only be captured into a
+    graph if its forward pass was.
     """
     clip_high = clip if clip_high is None else clip_high
     if not 0 <= clip <= 1 or not clip_high >= 0:

@@ -15,8 +15,9 @@ episode's end is of that kind.
 GPU tensors go through the HIP kernels (ops/src/selective.hip), which take
 float32 or bfloat16 inputs beside float32 parameters and keep the scan's state
 in float32.  CPU tensors take the eager path below, which is the kernels'
-oracle in tests.  The gradients cannot be differentiated again, and a backward
-pass can only be captured into a graph if its forward pass was.
+oracle in tests.  On the GPU the gradients cannot be differentiated again, there
+is no forward-mode derivative, and a backward pass can only be captured into a
+graph if its forward pass was.
 """
 
 import torch

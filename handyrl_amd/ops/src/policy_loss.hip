@@ -597,6 +597,11 @@ std::vector<torch::Tensor> clipped_policy_loss(
     const torch::Tensor& adv, const c10::optional<torch::Tensor>& mask,
     const c10::optional<torch::Tensor>& escale, double lo, double hi, double beta, double gamma)
 {
+    // a result without a forward-mode derivative would count as constant
+    for (const auto& t : {c10::make_optional(logits), c10::make_optional(old_lp),
+                          c10::make_optional(adv), mask, escale})
+        TORCH_CHECK_VALUE(!t || !t->_fw_grad(0).defined(),
+                          "clipped_policy_loss: has no forward-mode derivative on the GPU");
     TORCH_CHECK_VALUE(logits.is_cuda(), "clipped_policy_loss: logits must be on the GPU");
     TORCH_CHECK_VALUE(logits.scalar_type() == torch::kFloat32 ||
                       logits.scalar_type() == torch::kBFloat16,

@@ -1446,6 +1446,15 @@ void check_conv(const char* op, const Tensor& x, const Tensor& w, const OptTenso
     if (bias) check_like(op, "bias", *bias, x, torch::kFloat32, {x.size(-1)});
 }
 
+// The kernels give no forward-mode derivatives; a result without one would count
+// as constant.
+void check_forward_mode(const char* op, std::initializer_list<OptTensor> all)
+{
+    for (auto& t : all)
+        TORCH_CHECK_VALUE(!t || !t->_fw_grad(0).defined(), op,
+                          ": has no forward-mode derivative on the GPU");
+}
+
 bool wants_grad(std::initializer_list<OptTensor> all)
 {
     if (!at::GradMode::is_enabled()) return false;
@@ -1466,6 +1475,7 @@ std::vector<Tensor> causal_conv(const Tensor& x_in, const Tensor& w, const OptTe
                                 const OptTensor& state, const OptTensor& mask, bool silu)
 {
     const char* op = "causal_conv";
+    check_forward_mode(op, {x_in, w, bias, state});
     check_x(op, x_in, 3);
     check_conv(op, x_in, w, bias);
     if (state)
@@ -1484,6 +1494,7 @@ Tensor causal_conv_step(Tensor state, const Tensor& x_in, const Tensor& w, const
                         const OptTensor& mask, bool silu)
 {
     const char* op = "causal_conv_step";
+    check_forward_mode(op, {state, x_in, w, bias});
     check_x(op, x_in, 2);
     check_conv(op, x_in, w, bias);
     check_like(op, "state", state, x_in, x_in.scalar_type(),
@@ -1742,6 +1753,7 @@ std::vector<Tensor> selective_scan(
     const OptTensor& state, const OptTensor& mask)
 {
     const char* op = "selective_scan";
+    check_forward_mode(op, {x, dt, A, B, C, D, z, bias, state});
     check_x(op, x, 3);
     check_scan(op, x, dt, A, B, C, D, z, bias);
     if (state)
@@ -1766,6 +1778,7 @@ Tensor selective_step(Tensor state, const Tensor& x_in, const Tensor& dt_in, con
                       const OptTensor& mask)
 {
     const char* op = "selective_step";
+    check_forward_mode(op, {state, x_in, dt_in, A_in, B_in, C_in, D_in, z_in, bias_in});
     check_x(op, x_in, 2);
     check_scan(op, x_in, dt_in, A_in, B_in, C_in, D_in, z_in, bias_in);
     check_like(op, "state", state, x_in, torch::kFloat32,

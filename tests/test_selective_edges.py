@@ -5,9 +5,12 @@ test_selective.py."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
-from handyrl_amd.models.selective import selective_scan, selective_step
-from test_selective import STEP, make_scan, move, run_scan, scan_by_hand
+from handyrl_amd import ops
+from handyrl_amd.models.selective import (
+    causal_conv, causal_conv_step, selective_scan, selective_step)
+from test_selective import STEP, make_conv, make_scan, move, run_scan, scan_by_hand
 
 gpu = pytest.mark.gpu
 
@@ -76,3 +79,54 @@ def test_scan_forgets_at_once(rate, steps):
     selective_step(held, **row, **rest)
     assert held.isfinite().all()
     torch.testing.assert_close(held, last, rtol=64 * STEP, atol=64 * STEP * 10)
+
+
+def calls(device):
+    """Each operator's entry with its arguments, and those that carry derivatives."""
+    a, c = (move(make(2, 3, 8, 4)[0], device) for make in (make_scan, make_conv))
+    row = {k: v[:, 0] if k in ('x', 'dt', 'B', 'C', 'z', 'mask') else v for k, v in a.items()}
+    step = {k: v[:, 0] if k in ('x', 'mask') else v for k, v in c.items()}
+    scan = ('x', 'dt', 'A', 'B', 'C', 'D', 'z', 'dt_bias', 'state')
+    conv = ('x', 'weight', 'bias', 'state')
+    return [(selective_scan, a, scan), (selective_step, row, scan),
+            (causal_conv, c, conv), (causal_conv_step, step, conv)]
+
+
+def refuse_duals(device):
+    for call, args, names in calls(device):
+        for name in names:
+            with fwd.dual_level():
+                dual = fwd.make_dual(args[name].clone(), torch.ones_like(args[name]))
+                with torch.no_grad(), pytest.raises(ValueError, match='forward-mode'):
+                    call(**{**args, name: dual})
+        assert call(**args) is not None
+
+
+@pytest.mark.skipif(not ops.available(), reason='extension not built')
+def test_extension_refuses_forward_mode():
+    """The refusal comes before the extension looks at the device."""
+    ext = ops.require()
+    x = torch.zeros(2, 8)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError, match='causal_conv_step: has no forward-mode'):
+            ext.causal_conv_step(torch.zeros(2, 3, 8), dual, torch.zeros(8, 4), None, None, True)
+    with pytest.raises(ValueError, match='must be on the GPU'):
+        ext.causal_conv_step(torch.zeros(2, 3, 8), x, torch.zeros(8, 4), None, None, True)
+
+
+def test_eager_forward_mode():
+    """On the CPU the derivative is the formula's: as one step's difference of a linear map."""
+    a, _ = make_scan(2, 3, 8, 4)
+    a = move(a, double=True)
+    moved = torch.ones_like(a['x'])
+    with fwd.dual_level():
+        y, _ = selective_scan(**{**a, 'x': fwd.make_dual(a['x'], moved)})
+        got = fwd.unpack_dual(y).tangent
+    want = selective_scan(**{**a, 'x': a['x'] + moved})[0] - selective_scan(**a)[0]
+    torch.testing.assert_close(got, want, rtol=1e-10, atol=1e-10)
+
+
+@gpu
+def test_kernels_refuse_forward_mode():
+    refuse_duals('cuda')
