@@ -123,7 +123,7 @@ def clipped_policy_loss(logits, actions, old_log_probs, advantages, mask=None,
     (weighted by the mask), the number of clipped rows, and the mask's sum.
     On the GPU the gradient cannot be differentiated again, there is no
     forward-mode derivative, and a backward pass can only be captured into a
-    graph if its forward pass was.
+    graph if its forward pass was and no eager pass over the same logits lives on.
     """
     clip_high = clip if clip_high is None else clip_high
     if not 0 <= clip <= 1 or not clip_high >= 0:

@@ -17,7 +17,7 @@ float32 or bfloat16 inputs beside float32 parameters and keep the scan's state
 in float32.  CPU tensors take the eager path below, which is the kernels'
 oracle in tests.  On the GPU the gradients cannot be differentiated again, there
 is no forward-mode derivative, and a backward pass can only be captured into a
-graph if its forward pass was.
+graph if its forward pass was and no eager pass over the same inputs lives on.
 """
 
 import torch

@@ -24,7 +24,7 @@ def build(verbose=False):
     # `*_hip.hip` siblings next to the source, which a bare glob would pick
     # up on the next build (duplicate kernels / double op registration).
     sources = [os.path.join(src_dir, name)
-               for name in ('ext.hip', 'policy_loss.hip', 'selective.hip')]
+               for name in ('ext.hip', 'guards.hip', 'policy_loss.hip', 'selective.hip')]
 
     mod = cpp_extension.load(
         name='handyrl_amd_C',

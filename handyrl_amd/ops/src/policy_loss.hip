@@ -15,6 +15,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <hip/hip_runtime.h>
+#include "guards.h"
 
 namespace {
 
@@ -493,15 +494,6 @@ torch::Tensor as_rows(const torch::Tensor& logits)
     return flat.size(1) > 1 && flat.stride(1) != 1 ? flat.contiguous() : flat;
 }
 
-// The capture that a stream is in, or 0.
-unsigned long long capture_of(hipStream_t stream)
-{
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    C10_HIP_CHECK(hipStreamGetCaptureInfo(stream, &status, &id));
-    return status == hipStreamCaptureStatusActive ? id : 0;
-}
-
 std::vector<torch::Tensor> policy_forward(
     const torch::Tensor& logits, const torch::Tensor& action, const torch::Tensor& old_lp,
     const torch::Tensor& adv, const torch::Tensor& mask, const torch::Tensor& escale,
@@ -549,8 +541,8 @@ public:
         ctx->save_for_backward({logits, action, old_lp, adv, mask, escale});
         ctx->saved_data["coefs"] = std::vector<double>{lo, hi, beta, gamma};
         ctx->saved_data["grad"] = out[2];
-        ctx->saved_data["capture"] = (int64_t)capture_of(
-            at::cuda::getCurrentCUDAStream(logits.device().index()));
+        const c10::DeviceGuard guard(logits.device());
+        ctx->saved_data["capture"] = capture_now();
         ctx->mark_non_differentiable({out[1]});
         ctx->set_materialize_grads(false);
         return {out[0], out[1]};
@@ -568,16 +560,14 @@ public:
         const auto coefs = ctx->saved_data["coefs"].toDoubleVector();
         const c10::DeviceGuard guard(logits.device());
         hipStream_t stream = at::cuda::getCurrentCUDAStream();
+        const int64_t then = ctx->saved_data["capture"].toInt();
+        check_capture("clipped_policy_loss", then);
         torch::Tensor grad;
         if (!ctx->saved_data["grad"].isNone()) {
             grad = ctx->saved_data["grad"].toTensor();
             ctx->saved_data["grad"] = c10::IValue();
         }
-        const int64_t then = ctx->saved_data["capture"].toInt(), now = capture_of(stream);
-        // the leaves' own streams would be drawn into the capture and never joined
-        TORCH_CHECK(then != 0 || now == 0, "clipped_policy_loss: a captured backward pass needs "
-                    "a captured forward pass");
-        const bool ready = grad.defined() && then == now;
+        const bool ready = grad.defined() && then == capture_now();
         if (!ready) grad = torch::empty(logits.sizes(), logits.options());
         const auto flat = as_rows(logits);
         const auto up = grads[0].to(torch::kFloat32);
@@ -597,11 +587,7 @@ std::vector<torch::Tensor> clipped_policy_loss(
     const torch::Tensor& adv, const c10::optional<torch::Tensor>& mask,
     const c10::optional<torch::Tensor>& escale, double lo, double hi, double beta, double gamma)
 {
-    // a result without a forward-mode derivative would count as constant
-    for (const auto& t : {c10::make_optional(logits), c10::make_optional(old_lp),
-                          c10::make_optional(adv), mask, escale})
-        TORCH_CHECK_VALUE(!t || !t->_fw_grad(0).defined(),
-                          "clipped_policy_loss: has no forward-mode derivative on the GPU");
+    check_forward_mode("clipped_policy_loss", {logits, old_lp, adv, mask, escale});
     TORCH_CHECK_VALUE(logits.is_cuda(), "clipped_policy_loss: logits must be on the GPU");
     TORCH_CHECK_VALUE(logits.scalar_type() == torch::kFloat32 ||
                       logits.scalar_type() == torch::kBFloat16,

@@ -11,6 +11,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <hip/hip_runtime.h>
+#include "guards.h"
 
 namespace {
 
@@ -1259,23 +1260,6 @@ template <typename F> void by_type(const Tensor& x, F f)
 }
 template <int N> struct Const { static constexpr int value = N; };
 
-// The capture that the current stream is in, or 0.
-int64_t capture_now()
-{
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    C10_HIP_CHECK(hipStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(), &status, &id));
-    return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
-}
-
-// A captured backward pass of an eager forward pass would draw the leaves' own
-// streams into the capture, which never join it.
-void check_capture(const char* op, const torch::autograd::AutogradContext* ctx)
-{
-    TORCH_CHECK(ctx->saved_data.at("capture").toInt() != 0 || capture_now() == 0, op,
-                ": a captured backward pass needs a captured forward pass");
-}
-
 // A step changes the state behind torch's back: tell autograd's version check.
 void moved_on(const Tensor& state) {
     if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
@@ -1389,7 +1373,7 @@ public:
         auto saved = ctx->get_saved_variables();
         const auto &x = saved[0], &w = saved[1], &bias = saved[2], &state = saved[3];
         const c10::DeviceGuard guard(x.device());
-        check_capture("causal_conv", ctx);
+        check_capture("causal_conv", ctx->saved_data["capture"].toInt());
         auto stream = at::cuda::getCurrentCUDAStream();
         const int64_t taps = w.size(1);
         auto dy = grads[0].defined() ? grads[0].contiguous()
@@ -1444,15 +1428,6 @@ void check_conv(const char* op, const Tensor& x, const Tensor& w, const OptTenso
                       ": weight must be (channels, taps) with 2 to 4 taps, got ", w.sizes());
     check_like(op, "weight", w, x, torch::kFloat32, {x.size(-1), w.size(1)});
     if (bias) check_like(op, "bias", *bias, x, torch::kFloat32, {x.size(-1)});
-}
-
-// The kernels give no forward-mode derivatives; a result without one would count
-// as constant.
-void check_forward_mode(const char* op, std::initializer_list<OptTensor> all)
-{
-    for (auto& t : all)
-        TORCH_CHECK_VALUE(!t || !t->_fw_grad(0).defined(), op,
-                          ": has no forward-mode derivative on the GPU");
 }
 
 bool wants_grad(std::initializer_list<OptTensor> all)
@@ -1668,7 +1643,7 @@ public:
                  ctx->saved_data["softplus"].toBool()};
         const auto& ckpt = v[10];
         const c10::DeviceGuard guard(s.x.device());
-        check_capture("selective_scan", ctx);
+        check_capture("selective_scan", ctx->saved_data["capture"].toInt());
         auto stream = at::cuda::getCurrentCUDAStream();
         ScanArgs p = scan_args(s);
         auto fp32 = s.A.options();

@@ -41,3 +41,26 @@ def test_kernel_refuses_forward_mode(name):
         args[name] = fwd.make_dual(args[name], torch.ones_like(args[name]))
         with pytest.raises(ValueError, match='forward-mode'):
             clipped_policy_loss(**args, **COEFS)
+
+
+@gpu
+def test_captured_backward_beside_an_eager_graph():
+    """Refused while the eager graph of the same leaf lives, and right once it is gone."""
+    args = make((64,), 9, device='cuda')
+    leaf = args['logits'].requires_grad_()
+    kept = clipped_policy_loss(**args, **COEFS)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = clipped_policy_loss(**args, **COEFS)
+        with pytest.raises(RuntimeError, match='living eager graph'):
+            torch.autograd.grad(out[0], leaf)
+    want, = torch.autograd.grad(kept[0], leaf)
+    del kept, out, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(clipped_policy_loss(**args, **COEFS)[0], leaf)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

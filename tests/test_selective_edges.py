@@ -130,3 +130,29 @@ def test_eager_forward_mode():
 @gpu
 def test_kernels_refuse_forward_mode():
     refuse_duals('cuda')
+
+
+@gpu
+@pytest.mark.parametrize('which', ['scan', 'conv'])
+def test_captured_backward_beside_an_eager_graph(which):
+    """Refused while the eager graph of the same leaf lives, and right once it is gone."""
+    make, call = (make_scan, selective_scan) if which == 'scan' else (make_conv, causal_conv)
+    a, (dy, _) = make(2, 21, 16, 4)
+    a, dy = move(a, 'cuda'), dy.cuda()
+    leaf = a['x'].requires_grad_()
+    kept = call(**a)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(**a)
+        with pytest.raises(RuntimeError, match='living eager graph'):
+            torch.autograd.grad(out[0], leaf, dy)
+    want, = torch.autograd.grad(kept[0], leaf, dy)
+    del kept, out, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(call(**a)[0], leaf, dy)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
