@@ -1059,16 +1059,17 @@ __global__ __launch_bounds__(256, LOCAL ? 4 : 2) void scan_bwd_kernel(ScanArgs p
 
 // The rest of the backward pass in one launch, each block one part of it: sums
 // dB and dC over the channel tiles (and rounds them once), and dA, dD and dbias
-// over rows and segments, in a fixed order and 64 bits.
+// over rows and segments, in a fixed order and 64 bits.  `first` is the launch's
+// first part, where one launch cannot hold them all.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_finish_kernel(
     const float* __restrict__ bc, int tiles, long nbc, T* __restrict__ dB, T* __restrict__ dC,
     const float* __restrict__ dAp, const float* __restrict__ dDp, long rows, long nA, long nD,
-    float* __restrict__ dA, float* __restrict__ dD)
+    float* __restrict__ dA, float* __restrict__ dD, long first)
 {
     __shared__ double fold[16][17];
     const long blocks_bc = (nbc + 255) / 256;
-    long at = blockIdx.x;
+    long at = first + blockIdx.x;
     if (at < 2 * blocks_bc) {
         const bool second = at >= blocks_bc;
         const long i = (second ? at - blocks_bc : at) * 256 + threadIdx.x;
@@ -1246,10 +1247,13 @@ Tensor as_mask(const char* op, const OptTensor& mask, const Tensor& x)
     return (m.scalar_type() == torch::kBool ? m : m.ne(0)).contiguous();
 }
 
+// A launch counts its threads in 32 bits.
+constexpr int64_t kMostBlocks = (1LL << 24) - 1;
+
 int64_t blocks_for(int64_t threads, const char* op)
 {
     const int64_t n = (threads + 255) / 256;
-    TORCH_CHECK_VALUE(n < (1LL << 31), op, ": too large for one launch");
+    TORCH_CHECK_VALUE(n <= kMostBlocks, op, ": too large for one launch, share out the batch");
     return n;
 }
 
@@ -1326,18 +1330,18 @@ std::vector<Tensor> conv_forward(const Tensor& x, const Tensor& w, const Tensor&
     const c10::DeviceGuard guard(x.device());
     auto stream = at::cuda::getCurrentCUDAStream();
     const int64_t taps = w.size(1);
+    ConvArgs p = conv_args(x, w, bias, state, mask, silu);
+    const int channels = conv_channels(x, {state});
+    cut_conv(p, channels);
+    const int64_t n = blocks_for(p.batch * p.tiles * (p.width / channels), "causal_conv");
     auto y = torch::empty(x.sizes(), x.options());
     auto last = torch::empty({x.size(0), taps - 1, x.size(2)}, x.options());
-    ConvArgs p = conv_args(x, w, bias, state, mask, silu);
     if (p.batch == 0 || p.steps == 0) {
         if (state.defined()) last.copy_(state); else last.zero_();
         return {y, last};
     }
     p.y = y.data_ptr(); p.last = last.data_ptr();
-    const int channels = conv_channels(x, {state});
-    cut_conv(p, channels);
     by_conv(x, taps, channels, [&](auto t, auto k, auto v) {
-        const int64_t n = blocks_for(p.batch * p.tiles * (p.width / v.value), "causal_conv");
         if (p.mask)
             hipLaunchKernelGGL((conv_fwd_kernel<decltype(t), decltype(k)::value,
                                 decltype(v)::value, true>), dim3(n), dim3(256), 0, stream, p);
@@ -1569,9 +1573,7 @@ ScanArgs scan_args(const ScanIn& s)
 
 int64_t scan_blocks(const ScanArgs& p)
 {
-    const int64_t n = p.batch * p.segs * p.groups * p.tiles;
-    TORCH_CHECK_VALUE(n < (1LL << 31), "selective_scan: too large for one launch");
-    return n;
+    return blocks_for(p.batch * p.segs * p.groups * p.tiles * 256, "selective_scan");
 }
 
 // What the segments hand on: a state and the sum of their steps.
@@ -1591,6 +1593,7 @@ std::vector<Tensor> scan_forward(const ScanIn& s, bool train)
     const c10::DeviceGuard guard(s.x.device());
     auto stream = at::cuda::getCurrentCUDAStream();
     ScanArgs p = scan_args(s);
+    const int64_t blocks = scan_blocks(p);
     auto fp32 = s.A.options();
     auto y = torch::empty(s.x.sizes(), s.x.options());
     auto last = torch::empty({p.batch, p.width, p.states}, fp32);
@@ -1605,9 +1608,9 @@ std::vector<Tensor> scan_forward(const ScanIn& s, bool train)
     by_scan(s.x, lanes_for(p.states), [&](auto t, auto n) {
         if (p.segs > 1)
             hipLaunchKernelGGL((scan_fwd_kernel<decltype(t), decltype(n)::value, true>),
-                               dim3(scan_blocks(p)), dim3(256), 0, stream, p);
+                               dim3(blocks), dim3(256), 0, stream, p);
         hipLaunchKernelGGL((scan_fwd_kernel<decltype(t), decltype(n)::value, false>),
-                           dim3(scan_blocks(p)), dim3(256), 0, stream, p);
+                           dim3(blocks), dim3(256), 0, stream, p);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
     return {y, last, ckpt};
@@ -1689,10 +1692,13 @@ public:
             hipLaunchKernelGGL((scan_bwd_kernel<T, decltype(n)::value, false>),
                                dim3(scan_blocks(p)), dim3(256), 0, stream, p);
             const int64_t blocks = 2 * ((nb + 255) / 256) + (nA + 15) / 16 + (nD + 15) / 16;
-            hipLaunchKernelGGL(scan_finish_kernel<T>, dim3(blocks), dim3(256), 0, stream,
-                               p.dBp, (int)p.tiles, (long)nb, (T*)dB.data_ptr(), (T*)dC.data_ptr(),
-                               p.dAp, p.dDp, (long)rows, (long)nA, (long)nD,
-                               dA.data_ptr<float>(), dD.data_ptr<float>());
+            for (int64_t first = 0; first < blocks; first += kMostBlocks)
+                hipLaunchKernelGGL(scan_finish_kernel<T>,
+                                   dim3(std::min(kMostBlocks, blocks - first)), dim3(256), 0,
+                                   stream, p.dBp, (int)p.tiles, (long)nb, (T*)dB.data_ptr(),
+                                   (T*)dC.data_ptr(), p.dAp, p.dDp, (long)rows, (long)nA,
+                                   (long)nD, dA.data_ptr<float>(), dD.data_ptr<float>(),
+                                   (long)first);
         });
         C10_HIP_KERNEL_LAUNCH_CHECK();
         return out;

@@ -156,3 +156,45 @@ def test_captured_backward_beside_an_eager_graph(which):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@gpu
+def test_launches_past_their_limit():
+    """2^32 threads: refused before anything is allocated."""
+    x = torch.zeros(1, 1, 2048, device='cuda', dtype=torch.bfloat16).expand(1 << 22, 1, 2048)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    with pytest.raises(ValueError, match='causal_conv: too large for one launch'):
+        causal_conv(x, torch.zeros(2048, 4, device='cuda'))
+    x = x[:, :, :8]
+    for rows, groups in ((1 << 22, 8), (1 << 24, 1)):
+        b = torch.zeros(1, 1, 1, 1, device='cuda', dtype=x.dtype).expand(rows, 1, groups, 1)
+        u = x[:1].expand(rows, 1, 8)
+        with pytest.raises(ValueError, match='selective_scan: too large for one launch'):
+            selective_scan(u, u, -torch.ones(8, 1, device='cuda'), b, b)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+
+
+@gpu
+def test_gradients_of_more_parts_than_a_launch_holds():
+    """2^28 rates in the sums that finish the backward pass: as two halves of them."""
+    g = torch.Generator('cuda').manual_seed(0)
+    width = (1 << 22) + 64
+    r = lambda *s: torch.randn(*s, device='cuda', generator=g)
+    a = dict(x=r(1, 1, width), dt=r(1, 1, width).abs(), A=-r(width, 64).abs(), B=r(1, 1, 64),
+             C=r(1, 1, 64), D=r(width), state=r(1, width, 64))
+    dy, dlast = r(1, 1, width), r(1, width, 64)
+    got = run_scan(a, dy, dlast)
+    half = width // 2
+    for part in (slice(0, half), slice(half, width)):
+        cut = {k: v if k in 'BC' else v[part] if k in 'AD' else v[:, part] if k == 'state'
+               else v[:, :, part] for k, v in a.items()}
+        one = run_scan(cut, dy[:, :, part], dlast[:, part])
+        for k, v in one.items():
+            if k in ('x', 'dt', 'y'):
+                assert torch.equal(got[k][:, :, part], v), k
+            elif k in ('state', 'last'):
+                assert torch.equal(got[k][:, part], v), k
+            elif k in 'AD':
+                assert torch.equal(got[k][part], v), k
+        del one, cut
