@@ -141,6 +141,9 @@ class SelectiveCore(nn.Module):
     and carries ``hidden`` past the other steps.  Without gradient ``forward``
     takes the step kernels on a copy of ``hidden``; ``step_`` moves it on in
     place, for actors that keep it resident.
+
+    Parameters may be of any floating type: the operators take them, and carry
+    the scan's state, in 64 bits if they are that wide and in 32 bits otherwise.
     """
 
     def __init__(self, width, expand=2, states=16, taps=4, dt_rank=None):
@@ -163,18 +166,23 @@ class SelectiveCore(nn.Module):
     def init_hidden(self, batch_size=()):
         like = self.proj_in.weight
         return (like.new_zeros(*batch_size, self.taps - 1, self.inner),
-                like.new_zeros(*batch_size, self.inner, self.states, dtype=torch.float32))
+                like.new_zeros(*batch_size, self.inner, self.states, dtype=_real(like)))
 
     def _select(self, u):
         r, n = self.dt_rank, self.states
         dt, B, C = self.proj_select(u).split([r, n, n], -1)
-        return dict(x=u, dt=self.proj_dt(dt), A=-torch.exp(self.log_rate.float()), B=B, C=C,
-                    D=self.skip, dt_bias=self.dt_bias, dt_softplus=True)
+        real = _real(u)
+        return dict(x=u, dt=self.proj_dt(dt), A=-torch.exp(self.log_rate.to(real)), B=B, C=C,
+                    D=self.skip.to(real), dt_bias=self.dt_bias.to(real), dt_softplus=True)
+
+    def _taps(self, u):
+        real = _real(u)
+        return self.conv_weight.to(real), self.conv_bias.to(real)
 
     def window(self, x, hidden=None, mask=None):
         taken, state = (None, None) if hidden is None else hidden
         u, z = self.proj_in(x).chunk(2, -1)
-        u, last = causal_conv(u, self.conv_weight, self.conv_bias, activation='silu',
+        u, last = causal_conv(u, *self._taps(u), activation='silu',
                               state=None if taken is None else taken.to(u.dtype), mask=mask)
         y, state = selective_scan(**self._select(u), z=z, state=state, mask=mask)
         if taken is not None:
@@ -186,8 +194,7 @@ class SelectiveCore(nn.Module):
         with torch.no_grad():
             u, z = self.proj_in(x).chunk(2, -1)
             taken = hidden[0] if hidden[0].dtype == u.dtype else hidden[0].to(u.dtype)
-            u = causal_conv_step(taken, u, self.conv_weight, self.conv_bias, activation='silu',
-                                 mask=mask)
+            u = causal_conv_step(taken, u, *self._taps(u), activation='silu', mask=mask)
             if taken is not hidden[0]:
                 hidden[0].copy_(taken)
             y = selective_step(hidden[1], **self._select(u), z=z, mask=mask)

@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as fwd
 
 from handyrl_amd import ops
 from handyrl_amd.models.selective import (
-    causal_conv, causal_conv_step, selective_scan, selective_step)
+    SelectiveCore, causal_conv, causal_conv_step, selective_scan, selective_step)
 from test_selective import STEP, make_conv, make_scan, move, run_scan, scan_by_hand
 
 gpu = pytest.mark.gpu
@@ -198,3 +198,51 @@ def test_gradients_of_more_parts_than_a_launch_holds():
             elif k in 'AD':
                 assert torch.equal(got[k][part], v), k
         del one, cut
+
+
+def check_core_type(dtype, device):
+    """Parameters of another type, against a core in 64 bits that holds the same
+    values.  Some nine roundings to `dtype` stand between an input and its output
+    (projections, convolution, B, C, dt, y), each of half a step, and what follows
+    makes at most twice as much of it (the slopes of silu and softplus are below
+    1.1, products take two factors): 18 half steps of the outputs' size; for
+    sums over 32 bits inside as many again."""
+    torch.manual_seed(0)
+    core = SelectiveCore(24, states=8).to(device).to(dtype)
+    exact = SelectiveCore(24, states=8).double()
+    exact.load_state_dict({k: v.double().cpu() for k, v in core.state_dict().items()})
+    x = torch.randn(6, 17, 24, device=device, dtype=dtype)
+    mask = torch.rand(6, 17, device=device) < 0.8
+    hidden = core.init_hidden([6])
+    real = torch.float64 if dtype == torch.float64 else torch.float32
+    assert hidden[0].dtype == dtype and hidden[1].dtype == real
+    y, end = core.window(x, hidden, mask)
+    assert y.dtype == end[0].dtype == dtype and end[1].dtype == real
+    want, last = exact.window(x.double().cpu(), exact.init_hidden([6]), mask.cpu())
+    y.float().square().sum().backward()
+    want.square().sum().backward()
+    half = torch.finfo(dtype).eps / 2
+    near = lambda a, b, k: (a.double().cpu() - b).norm() <= (k * half + 1e-6) * b.norm()
+    assert near(y, want, 36) and near(end[0], last[0], 36) and near(end[1], last[1], 36)
+    for (name, p), q in zip(core.named_parameters(), exact.parameters()):
+        # y^2 doubles what y is off by, and the gradient walks the same way back
+        assert p.grad.dtype == dtype and near(p.grad, q.grad, 108), name
+    with torch.no_grad():
+        held = core.init_hidden([6])
+        for t in range(17):
+            one = core.step_(x[:, t], held, mask[:, t])
+            assert one.dtype == dtype
+            assert near(one[mask[:, t]], want[:, t][mask[:, t].cpu()], 72)
+        assert near(held[0], last[0], 36) and near(held[1], last[1], 36)
+        assert core(x[:, 0])[0].dtype == dtype
+
+
+@pytest.mark.parametrize('dtype', [torch.float64, torch.float32, torch.bfloat16, torch.float16])
+def test_core_type(dtype):
+    check_core_type(dtype, 'cpu')
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_kernel_core_type(dtype):
+    check_core_type(dtype, 'cuda')
