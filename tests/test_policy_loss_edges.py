@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as fwd
 
 from handyrl_amd import ops
 from handyrl_amd.losses import clipped_policy_loss
-from test_policy_loss import COEFS, make
+from test_policy_loss import COEFS, assert_matches_64_bits, make
 
 gpu = pytest.mark.gpu
 
@@ -64,3 +64,23 @@ def test_captured_backward_beside_an_eager_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+# the widths at which another kernel takes over, and the last of each: lanes a row
+# and values a lane up to 1024, then 16 byte pieces a lane up to 8192 pieces a row
+BORDERS = [16, 17, 31, 32, 33, 128, 129, 256, 257, 512, 513, 1000, 1024, 1025,
+           2051, 2052, 4099, 4100, 4103, 4104, 8192, 8195, 8196, 8199, 8200, 12001, 16387, 16388,
+           16391, 16392, 32771, 32772, 32775, 32776, 40001, 65543, 65544]
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('width', BORDERS)
+def test_kernels_at_their_borders(width, dtype):
+    assert_matches_64_bits(make((7,), width, dtype=dtype, device='cuda'))
+    assert_matches_64_bits(make((3,), width, seed=1, dtype=dtype, legal=0.3, device='cuda'), grad_out=-1.7)
+    args = make((5,), width, seed=2, dtype=dtype, device='cuda')
+    wide = torch.zeros(5, width + 5, dtype=dtype, device='cuda')
+    wide[:, 3:-2] = args['logits']                  # rows that begin anywhere between 16 byte borders
+    args['logits'] = wide[:, 3:-2]
+    assert_matches_64_bits(args)

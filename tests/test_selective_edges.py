@@ -3,6 +3,8 @@ growth past a float's range, rates without bound, plans of several chunks a
 segment and of several rows a lane.  Helpers and tolerances are those of
 test_selective.py."""
 
+import threading
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -10,7 +12,8 @@ import torch.autograd.forward_ad as fwd
 from handyrl_amd import ops
 from handyrl_amd.models.selective import (
     SelectiveCore, causal_conv, causal_conv_step, selective_scan, selective_step)
-from test_selective import STEP, make_conv, make_scan, move, run_scan, scan_by_hand
+from test_selective import (
+    STEP, assert_conv, assert_scan, make_conv, make_scan, move, run_scan, scan_by_hand)
 
 gpu = pytest.mark.gpu
 
@@ -246,3 +249,115 @@ def test_core_type(dtype):
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_kernel_core_type(dtype):
     check_core_type(dtype, 'cuda')
+
+
+# ---- steps of so many rows that a lane takes several: from 2^20 lanes (scan) and
+# 2^20 values (convolution) on
+
+def row_mask(kind, batch):
+    return dict(none=None, alternate=torch.arange(batch) % 2 == 1, runs=torch.arange(batch) % 7 < 3,
+                few=torch.arange(batch) % 64 == 63)[kind]
+
+
+def check_rows(state, before, y, mask):
+    """Rows of mask 0 keep every bit of their state and give 0."""
+    if mask is not None:
+        assert torch.equal(state[~mask], before[~mask]) and (y[~mask] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('kind', ['none', 'alternate', 'runs', 'few'])
+@pytest.mark.parametrize('batch, width, states, groups', [
+    (4099, 64, 16, 1), (8191, 33, 16, 3), (4099, 128, 5, 2), (8191, 40, 13, 1), (4097, 17, 64, 1)])
+def test_scan_steps_of_many_rows(batch, width, states, groups, kind, dtype):
+    a, (dy, dlast) = make_scan(batch, 1, width, states, groups, share=1.0, dtype=dtype)
+    if (mask := row_mask(kind, batch)) is not None:
+        a['mask'] = mask[:, None]
+    y, last = selective_scan(**move(a, double=True))
+    size = scan_by_hand(a, dy, dlast, absolute=True)
+    row = {k: v[:, 0] if k in ('x', 'dt', 'B', 'C', 'z', 'mask') else v for k, v in move(a, 'cuda').items()}
+    held = row['state'].clone()
+    got = selective_step(**{**row, 'state': held})
+    check_rows(held, row['state'], got, row.get('mask'))
+    assert_results(dict(y=got[:, None], last=held), dict(y=y, last=last), size, a)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('kind', ['none', 'alternate', 'runs', 'few'])
+@pytest.mark.parametrize('batch, width, taps', [(4099, 256, 4), (8191, 129, 3), (8190, 130, 2)])
+def test_conv_steps_of_many_rows(batch, width, taps, kind, dtype):
+    a, _ = make_conv(batch, 1, width, taps, share=1.0, dtype=dtype)
+    mask = row_mask(kind, batch)
+    row = {k: v[:, 0] if k == 'x' else v for k, v in a.items()}
+    wide = move(row, double=True)
+    want = wide['state'].clone()
+    y = causal_conv_step(**{**wide, 'state': want}, mask=mask)
+    row = move(row, 'cuda')
+    held = row['state'].clone()
+    got = causal_conv_step(**{**row, 'state': held}, mask=None if mask is None else mask.cuda())
+    check_rows(held, row['state'], got, None if mask is None else mask.cuda())
+    assert torch.equal(held.double().cpu(), want)           # inputs move on as they are
+    terms = torch.cat([wide['state'], wide['x'][:, None]], 1).abs() * wide['weight'].abs().t()
+    # a few operations on each term; silu moves by at most 1.1 of what it takes
+    tol = STEP * 24 * 1.1 * (terms.sum(1) + wide['bias'].abs()) + torch.finfo(dtype).eps / 2 * y.abs()
+    assert ((got.double().cpu() - y).abs() <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('case', [
+    dict(batch=1, steps=1100, width=24, states=16),             # 35 segments of 2 chunks, the last of 1
+    dict(batch=1, steps=3300, width=6, states=3, groups=2),     # 52 of 4, the last of 3
+    dict(batch=2, steps=1500, width=20, states=30, share=1.0, gate=False),      # 47 of 2
+    dict(batch=12, steps=940, width=33, states=36),             # 20 of 3, the last of 2, 3 tiles
+    dict(batch=6, steps=2100, width=70, states=8, groups=2, state=False, plain=True)])   # 44 of 3
+def test_segments_of_several_chunks(case, dtype):
+    a, grads = make_scan(dtype=dtype, **case)
+    assert_scan(a, *grads)
+
+
+@gpu
+@pytest.mark.parametrize('case', [
+    # more items than parts: a lane walks several
+    dict(batch=300, steps=100, width=6, taps=4), dict(batch=300, steps=100, width=5, taps=3, share=0.2),
+    dict(batch=40, steps=130, width=1030, taps=2, share=1.0, state=False),
+    # 2^18 lanes: tiles of 32 and 64 steps, the last one short, two channels a lane and one
+    dict(batch=100, steps=130, width=1200, taps=4), dict(batch=100, steps=130, width=1752, taps=4, share=0.2),
+    dict(batch=64, steps=130, width=1367, taps=3), dict(batch=64, steps=167, width=1367, taps=4, share=1.0)])
+def test_conv_of_many_tiles(case):
+    dtype = torch.bfloat16 if case['taps'] == 4 else torch.float32
+    a, grads = make_conv(dtype=dtype, **case)
+    assert_conv(a, *grads)
+
+
+@gpu
+def test_eager_passes_while_another_thread_captures():
+    """As the learner trains while an actor thread captures its graph."""
+    made = [make_scan(2, 40, 32, 8, seed=s) for s in (0, 1)]
+    (a, dy, dlast), (b, ey, elast) = (
+        (move(a, 'cuda'), dy.cuda(), dlast.cuda()) for a, (dy, dlast) in made)
+    want, there = run_scan(a, dy, dlast), run_scan(b, ey, elast)
+    got, failed = [], []
+
+    def train():
+        try:
+            got.extend(run_scan(a, dy, dlast) for _ in range(3))
+        except Exception as e:          # noqa: BLE001 - raised again below
+            failed.append(e)
+
+    thread = threading.Thread(target=train)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode='thread_local'):
+        one = run_scan(b, ey, elast)
+        thread.start()
+        thread.join()
+        two = run_scan(b, ey, elast)
+    assert not failed, failed
+    graph.replay()
+    torch.cuda.synchronize()
+    for run in got:
+        assert all(torch.equal(run[k], v) for k, v in want.items())
+    for run in (one, two):
+        assert all(torch.equal(run[k], v) for k, v in there.items())
