@@ -361,3 +361,26 @@ def test_eager_passes_while_another_thread_captures():
         assert all(torch.equal(run[k], v) for k, v in want.items())
     for run in (one, two):
         assert all(torch.equal(run[k], v) for k, v in there.items())
+
+
+@gpu
+def test_scan_past_32_bit_offsets_to_the_bit():
+    """2.4e9 values a tensor.  Three rows are cut as one is, 64 segments of 1024
+    chunks, so the last row gives every bit that it gives alone."""
+    shape = (3, 1 << 20, 768)
+    g = torch.Generator('cuda').manual_seed(0)
+    wide = torch.randn(shape[1:], device='cuda', generator=g).bfloat16()
+    x = torch.empty(shape, device='cuda', dtype=torch.bfloat16)
+    for b in range(3):
+        x[b] = wide.roll(b, 0)
+    A = -torch.rand(768, 2, device='cuda', generator=g) - 0.5
+    B = torch.randn(3, shape[1], 2, device='cuda', generator=g).bfloat16()
+
+    def run(x, B):
+        leaves = x.detach().requires_grad_(), B.detach().requires_grad_()
+        y, last = selective_scan(leaves[0], x, A, leaves[1], B, dt_softplus=True)
+        return y.detach(), last.detach(), *torch.autograd.grad(y, leaves, x)
+
+    alone = run(x[2:], B[2:])
+    for a, b in zip(run(x, B), alone):
+        assert torch.equal(a[2:], b)
