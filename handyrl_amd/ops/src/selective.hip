@@ -433,7 +433,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p)
 }
 
 // One step of up to CU rows a lane, which then share its taps: 8192 x 512 bf16
-// with every other row observed takes 8.1 us against 15.4 with a row a lane
+// with every other row observed takes 8.3 us against 15.4 with a row a lane
 // (33.6 MB; a copy of as much takes 6.6).
 template <typename T, int K, int V>
 __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs p)
@@ -700,7 +700,8 @@ __device__ __forceinline__ void load_channels(const float* from, const Place<L>&
 // h e^(ln2 p).  A whole segment's factor may pass the range of a float where its
 // product with a small state, or one of 0, does not, so p's whole part goes to the
 // exponent of the product; behind 600 the product of any float but 0 has left the
-// range.  A p that is not a number comes back in `e` below.
+// range.  A p that is not a number comes back in `e` below.  This costs 4 of the
+// 114 us that the walk of 4x2048x2048 takes, 1.5 of 68 for 1x8192x1024.
 __device__ __forceinline__ float grown(float h, float p) {
     p = fminf(fmaxf(p, -600.f), 600.f);
     const float whole = rintf(p);
@@ -739,8 +740,8 @@ struct StepIn {
 // segments behind it.  Otherwise the outputs, from the state before the
 // segment: the carried one moved through the segments before.  Vector
 // instructions bound both: 17 and 23 a step of four states, and 0.3 as many to
-// stage a chunk.  4x2048x2048 with 16 states, 8 segments: 64 and 110 us (of the
-// memory's rate they take 0.5 and 2.6 TB/s).
+// stage a chunk.  4x2048x2048 with 16 states, 8 segments: 65 and 114 us (of the
+// memory's rate they take 0.5 and 2.5 TB/s).
 template <typename T, int L, bool LOCAL>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
 {
@@ -837,7 +838,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs p)
 // LOCAL: a segment's carry from a zero one behind it.  Otherwise the
 // gradients: h is walked again from a kept state and stays in registers with
 // exp(d A), then the same steps are walked backwards.  4x2048x2048 with 16
-// states, 8 segments: 74 and 322 us; of the latter's issue slots vector
+// states, 8 segments: 74 and 327 us; of the latter's issue slots vector
 // instructions take 65 to 70 %, a fifth of them to stage and to store a chunk.
 // Eight steps of states and decays at a time stay below 256 registers: 593 us
 // for training 4x2048x2048 against 633 with sixteen, which spill.
@@ -1129,8 +1130,9 @@ constexpr int SR = 2;           // rows that a lane of a large step has in fligh
 // One step: four states a lane, L lanes a channel, the state in place.  What
 // bounds it is the state's way to the lane and back.  8192 x 512 x 16 with every
 // other row observed (286 MB): 114 us with a row a lane, 102 with two, 85 with
-// the masks read first and the state past the caches (105 with one row); four
-// rows a lane take 91, for their registers take waves.
+// the masks read first and the state past the caches (105 with one row; these as
+// replayed graphs: a launch among others takes the last 79); four rows a lane
+// take 91, for their registers take waves.
 template <typename T, int L>
 __global__ __launch_bounds__(256) void scan_step_kernel(StepArgs p)
 {
